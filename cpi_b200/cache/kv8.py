@@ -1,0 +1,101 @@
+"""The cache in 8 bits: its tensors, and the pages that a step of several tokens works on.
+
+Positions 64 b .. 64 b + 63 of a sequence are its block b, one page.  A complete block is held as codes of 8 bits with one
+power of two as scale per page and key/value head, keys and values each (an element stands for code * scale); the block of
+the newest position is held in bfloat16, in the sequence's *tail*, until it is complete.  A query sees the keys and values
+of its own block in bfloat16 and those of earlier blocks as held in 8 bits, whatever step brought them: a position's result
+does not depend on how its sequence was cut into steps.
+
+  "int8"   scale = the smallest power of two with max |x| <= 127 scale; code = x / scale to the nearest integer
+  "e4m3"   max |x| / scale in [128, 256); code = x / scale to the nearest e4m3 number
+
+int8 is finer for numbers of like size; e4m3 keeps the relative precision of small numbers in a block with large ones.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import numpy as np
+import torch
+
+BLOCK = 64                       # positions of a block, and of a page
+FORMATS = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+
+
+class Kv8Cache(NamedTuple):
+    """One layer's cache.  Pages are shared by the slots through a page table; tails belong to slots."""
+    k: torch.Tensor              # int8 or float8_e4m3fn [pages, kv heads, 64, head_dim]
+    v: torch.Tensor
+    k_scale: torch.Tensor        # float32 [pages, kv heads], powers of two
+    v_scale: torch.Tensor
+    k_tail: torch.Tensor         # bfloat16 [slots, kv heads, 64, head_dim]: row p % 64 is position p of the slot's newest block
+    v_tail: torch.Tensor
+
+
+def needed_blocks(start: int, new: int, window_kind: str, window_size: int, keep_first: int) -> list:
+    """The blocks that a step of `new` tokens from position `start` reads in 8 bits: those before the last token's own
+    that its first token's window, or the kept first positions, reach."""
+    low = 0
+    if window_kind == "chunk":
+        low = start // window_size * window_size
+    elif window_kind == "sliding":
+        low = max(0, start - window_size + 1)
+    keep = keep_first if window_kind == "sliding" else 0
+    own = (start + new - 1) // BLOCK
+    first = low // BLOCK
+    return list(range(min(-(-keep // BLOCK), first))) + list(range(first, own))
+
+
+class Kv8Plan:
+    """Where a step's tokens and the blocks that they see lie among the step's own bfloat16 pages.  Made once per step and
+    window (`starts`, `n_new`, `slots` per sequence, as in a StepBatch), used by every layer with that window.
+
+    Pages 0 .. n_earlier - 1 hold earlier blocks; pages n_earlier .. n_pages - 1 the blocks that the step's tokens fall into,
+    sequence after sequence from each one's first new block on.  `exact_table` and `earlier_table` [sequences, width] name
+    them per block (-1: none); a kernel that stores rows through a page table stores them through `exact_table` with
+    `seq_ids` as the sequences' slots."""
+
+    def __init__(self, starts, n_new, slots, *, window_kind: str = "full", window_size: int = 0, keep_first: int = 0, device="cuda"):
+        if not len(starts) == len(n_new) == len(slots) or not len(starts):
+            raise ValueError("Kv8Plan: a start, a number of tokens and a slot per sequence")
+        if min(n_new) < 1 or min(starts) < 0 or min(slots) < 0:
+            raise ValueError("Kv8Plan: sequences bring a token or more, from position 0 on")
+        if window_kind not in ("full", "chunk", "sliding") or (window_kind != "full" and window_size < 1):
+            raise ValueError(f"Kv8Plan: window '{window_kind}' of {window_size}")
+        if len(set(slots)) != len(slots):
+            raise ValueError("Kv8Plan: a slot is named twice")
+        n = len(starts)
+        self.n_seqs, self.n_tokens = n, int(sum(n_new))
+        self.window = (window_kind, int(window_size) if window_kind != "full" else 0, int(keep_first) if window_kind == "sliding" else 0)
+        ends = [s + m for s, m in zip(starts, n_new)]
+        self.width = max(-(-e // BLOCK) for e in ends)
+        tables = np.full((2, n, self.width), -1, dtype=np.int32)        # [earlier, exact]
+        self.n_earlier = 0
+        for i, (s, m) in enumerate(zip(starts, n_new)):
+            blocks = needed_blocks(s, m, *self.window)
+            tables[0, i, blocks] = np.arange(self.n_earlier, self.n_earlier + len(blocks))
+            self.n_earlier += len(blocks)
+        at = self.n_earlier
+        jobs = []
+        for i, (s, e) in enumerate(zip(starts, ends)):
+            first, n_blocks = s // BLOCK, -(-e // BLOCK)
+            tables[1, i, first:n_blocks] = np.arange(at, at + n_blocks - first)
+            last_rows = e - (n_blocks - 1) * BLOCK
+            for b in range(first, n_blocks):
+                keeps_tail = b == first
+                jobs.append((slots[i], b, s - b * BLOCK if b == first else 0, min(BLOCK, e - b * BLOCK), tables[0, i, b], at + b - first,
+                             at + n_blocks - 1 - first if keeps_tail else -1, last_rows))
+            at += n_blocks - first
+        for i, s in enumerate(starts):
+            for b in np.flatnonzero(tables[0, i, :s // BLOCK] >= 0):
+                jobs.append((slots[i], b, 0, BLOCK, tables[0, i, b], -1, -1, 0))
+        self.n_pages, self.n_jobs = at, len(jobs)
+        flat = np.concatenate([tables.ravel(), np.arange(n, dtype=np.int32), np.asarray(jobs, dtype=np.int32).ravel()])
+        host = torch.from_numpy(flat)
+        dev = torch.device(device)
+        if dev.type == "cuda":
+            host = host.pin_memory()           # (kept below: the copy reads it until it has run)
+        self._host, words = host, n * self.width
+        d = host.to(dev, non_blocking=True)
+        self.earlier_table, self.exact_table = d[:words].view(n, -1), d[words:2 * words].view(n, -1)
+        self.seq_ids, self.jobs = d[2 * words:2 * words + n], d[2 * words + n:]

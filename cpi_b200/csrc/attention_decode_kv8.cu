@@ -1,0 +1,673 @@
+// Decode attention over the cache in 8 bits (kv8.cuh): one new token per sequence, its own block of 64 positions in bfloat16 (the
+// sequence's tail), the complete blocks before it as codes with a scale per block and head.
+//
+// A block of threads serves one (split, key/value head, token).  A fifth warp streams (page, head) tiles of codes (64 x D bytes of
+// keys, as many of values; TMA boxes of 128 bytes with the 128-byte swizzle) into a ring of shared-memory stages; four warps take
+// 16 positions of each tile and run an online softmax of their own:
+//     S^T = K Q^T     m16n8k16 with the positions as M and the group's heads as N (8, or twice 8): with heads as M half of the
+//                     rows would be empty in the usual groups of 4 to 8, and a lane then holds the maxima of the heads that its
+//                     outputs belong to.  The codes become float16 in registers: an int8 c as 1024 + (c + 128) by putting its byte
+//                     under the exponent of 1024, less 1152; e4m3 by the hardware's conversion; both exact.  Which positions of k
+//                     a lane's bytes fill is free as long as Q's do the same, so four neighbouring bytes of a row need no shuffle.
+//     O^T += V^T P^T  values by transposing loads: a pair of bytes is a pair of features, even features form the upper half of
+//                     M, odd ones the lower.  P^T comes out of S^T's registers by movmatrix.
+// The queries are float16 too, each head's divided by a power of two (11 bits of significand hold bfloat16's 8 exactly; what is
+// 2^-22 below a head's largest element loses bits).  Scales act on scores in float32; the value scale 2^e enters the exponent: a
+// probability is p = 2^(s + e - m) with m the maximum of s + e, and the sum takes p 2^-e.  So blocks of any scale share one
+// accumulator, at no operation per output.
+// p is rounded to float16 (11 bits) against a reference m that is raised when s + e has outgrown it by 2^8: p <= 2^14, and what
+// is 2^-20 of the largest still has all its bits.  Sums, maxima and outputs are float32.
+//
+// The tail: each warp takes 16 positions in bfloat16, straight from memory (one page at most, in the last split).  A token that
+// completes its block (position 63 of 64) has its tail turned into codes by the threads that serve it, for the steps after this one.
+// Rows of masked positions are zeros before they are multiplied: what an earlier sequence left cannot reach a result.
+// Waits are bounded as in attention_decode.cu.
+#include "kv8.cuh"
+#include <cuda.h>
+
+namespace cpi {
+namespace tc {
+int get_map_2d_bf16(const void* ptr, uint64_t inner, uint64_t rows, uint64_t row_stride_bytes, uint32_t box_inner,
+                    uint32_t box_rows, CUtensorMap* out);
+}
+namespace dec8 {
+
+using kv8::PAGE;
+constexpr int NT = 160, CONSUMERS = 4;
+constexpr uint32_t kSpinLimit = 1u << 24;
+constexpr float kSlack = 8.f, kLift = 6.f;        // p = 2^(s + e - m + kLift), m raised when s + e exceeds it by kSlack
+constexpr int kTailUnits = 2;                     // a tail's bytes, in pages of codes
+constexpr int kMaxSplits = 256;
+
+struct Params {
+  const __nv_bfloat16* q; __nv_bfloat16* out;     // [T, NH, D]
+  const float *k_scale, *v_scale;                 // [n_pages, NKV]
+  const __nv_bfloat16 *k_tail, *v_tail;           // [n_slots, NKV, 64, D]
+  uint8_t *k, *v; float *k_scale_w, *v_scale_w;   // what a completed block is written to
+  const int* page_table; int max_blocks, n_pages, n_slots, n_seqs;
+  const int *token_seq, *token_pos, *seq_slot;
+  int n_heads, n_kv_heads;
+  int window_kind, window_size, keep_first;
+  float scale_log2, cap_in, cap_out;              // soft cap c > 0: scale / c and c log2(e); else 0
+  int n_splits;
+  float* part_o; float2* part_ml;                 // [T, NH, splits, D], [T, NH, splits]
+  const float* sink;
+  int* error_flag;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+// false when the wait ran out here or in another warp
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* aborted) {
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 255u && *aborted) return false;
+  }
+  *aborted = 1;
+  return false;
+}
+__device__ __forceinline__ void tma_load_2d(void* smem, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(smem_u32(smem)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t s) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t s) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s) : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ int window_low(int kind, int size, int pos) {
+  if (kind == 1) return (pos / size) * size;
+  if (kind == 2) return max(0, pos - size + 1);
+  return 0;
+}
+// 2^(sink - m), in the units of p; a sink far above every score gives a huge finite sum
+__device__ __forceinline__ float sink_term(const float* sink, int head, float m) {
+  return sink ? exp2f(fminf(sink[head] * 1.4426950408889634f - m + kLift, 120.f)) : 0.f;
+}
+// A barrier of the four consumer warps; whether any of their threads brought `v`.
+__device__ __forceinline__ bool any_consumer(bool v) {
+  int r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.or.pred.aligned q, 1, 128, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+               : "=r"(r) : "r"((int)v) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void consumers_sync() { asm volatile("barrier.cta.sync.aligned 1, 128;" ::: "memory"); }
+// The four codes of a word as two pairs of float16: bytes (0, 1) and (2, 3), or with SPLIT bytes (0, 2) and (1, 3).
+template <int FMT, bool SPLIT> __device__ __forceinline__ void numbers(uint32_t w, uint32_t& a, uint32_t& b) {
+  if (FMT == kv8::kInt8) {
+    w ^= 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));              // 1024 + 128
+    uint32_t x = __byte_perm(w, 0x64646464u, SPLIT ? 0x4240 : 0x4140), y = __byte_perm(w, 0x64646464u, SPLIT ? 0x4341 : 0x4342);
+    __half2 u = __hsub2(*reinterpret_cast<__half2*>(&x), off), v = __hsub2(*reinterpret_cast<__half2*>(&y), off);
+    a = *reinterpret_cast<uint32_t*>(&u);
+    b = *reinterpret_cast<uint32_t*>(&v);
+  } else {
+    if (SPLIT) w = __byte_perm(w, 0u, 0x3120);
+    a = kv8::e4m3x2_f16x2((uint16_t)w);
+    b = kv8::e4m3x2_f16x2((uint16_t)(w >> 16));
+  }
+}
+
+template <int D> struct Shape {
+  static constexpr int TILE = PAGE * D;                     // bytes of a (page, head) tile of codes
+  static constexpr int STAGES = D == 128 ? 4 : 6;
+  static constexpr int LINES = TILE / 128;                  // the tile as lines of 128 bytes (one, or half, a position each)
+  static constexpr int RING = STAGES * 2 * TILE;
+};
+// Byte offset of the 16-byte chunk `c` of position `row` in a tile, as the copy engine's 128-byte swizzle leaves it.
+template <int D> __device__ __forceinline__ uint32_t chunk_at(int row, int c) {
+  const int at = row * (D / 16) + c, line = at >> 3;
+  return (uint32_t)(line * 128 + (((at & 7) ^ (line & 7)) << 4));
+}
+
+template <int D, int FMT, int HT>
+__global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) attention_decode_kv8_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                                   const __grid_constant__ CUtensorMap map_v, Params p) {
+  using S = Shape<D>;
+  constexpr int STAGES = S::STAGES, NC = D / 16;            // NC: 16-byte chunks of a row, steps of k, tiles of M
+  extern __shared__ uint8_t smem_dyn[];
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES];
+  __shared__ float wm[CONSUMERS][HT * 8], wl[CONSUMERS][HT * 8];
+  __shared__ uint32_t top_s[2][CONSUMERS];
+  __shared__ int abort_s;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  const int split = blockIdx.x, kvh = blockIdx.y, t = blockIdx.z;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* aborted = &abort_s;
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], CONSUMERS); }
+    abort_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();                                  // (in this order: it reads cached rows, see common.cuh)
+
+  const int G = p.n_heads / p.n_kv_heads;
+  int pos = p.token_pos[t];
+  const int seq = p.token_seq[t];
+  int slot = seq >= 0 && seq < p.n_seqs ? p.seq_slot[seq] : -1;
+  // a position below zero is a padded row: it sees nothing and its output is zero
+  if (pos >= 0 && (slot < 0 || slot >= p.n_slots || pos / PAGE >= p.max_blocks)) {
+    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+    pos = -1;
+  }
+  const int lo = pos < 0 ? 0 : window_low(p.window_kind, p.window_size, pos);
+  const int* table = p.page_table + (size_t)max(slot, 0) * p.max_blocks;
+  // The complete blocks that hold visible positions: kept ones (0 .. n_kept - 1), then the window's, b_lo .. own - 1.
+  const int b_lo = lo / PAGE, own = pos < 0 ? 0 : pos / PAGE;
+  const int keep = p.window_kind == 2 ? p.keep_first : 0;
+  const int n_kept = min((keep + PAGE - 1) / PAGE, b_lo);
+  const int n_items = pos < 0 ? 0 : n_kept + own - b_lo;
+  auto block_of = [&](int i) { return i < n_kept ? i : b_lo + i - n_kept; };
+  const int per = (n_items + kTailUnits + p.n_splits - 1) / p.n_splits;
+  const int begin = min(n_items, split * per), end = split == p.n_splits - 1 ? n_items : min(n_items, begin + per);
+  const bool has_tail = pos >= 0 && split == p.n_splits - 1;
+  const int total_pages = p.n_pages;
+
+  if (warp == CONSUMERS) {
+    // ---- the producer: page numbers 32 at a time, then a tile of keys and one of values per item ----
+    int pages = 0;
+    for (int i = begin; i < end; ++i) {
+      const int n = i - begin, st = n % STAGES;
+      if ((n & 31) == 0) {
+        const int at = i + lane;
+        pages = at < end ? table[block_of(at)] : 0;
+        if (pages < 0 || pages >= total_pages) {            // (beyond the map's last row: zeros arrive)
+          pages = total_pages;
+          if (p.error_flag) atomicExch(p.error_flag, 3);
+        }
+      }
+      const int page = __shfl_sync(0xffffffffu, pages, n & 31);
+      int ok = 1;
+      if (lane == 0) {
+        if (n >= STAGES) ok = mbar_wait(&empty_bar[st], ((n / STAGES) - 1) & 1, aborted);
+        if (ok) {
+          const int line = (page * p.n_kv_heads + kvh) * S::LINES;
+          mbar_expect_tx(&full_bar[st], 2 * S::TILE);
+          tma_load_2d(ring + st * 2 * S::TILE, &map_k, &full_bar[st], 0, line);
+          tma_load_2d(ring + st * 2 * S::TILE + S::TILE, &map_v, &full_bar[st], 0, line);
+        }
+      }
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+    }
+  } else {
+    // ---- the consumers ----
+    const int g = lane >> 2, j = lane & 3;
+    const int key0 = warp * 16;
+    const __nv_bfloat16* q = p.q + ((size_t)t * p.n_heads + (size_t)kvh * G) * D;
+    // B operands: column g = head g of the tile (heads beyond the group are zeros), k in the order of a lane's bytes
+    uint32_t qf[HT][NC][2];
+    float f[HT][2];                                         // per head of this lane's columns 2j, 2j + 1: 2^(q's power) scale log2(e)
+#pragma unroll
+    for (int h = 0; h < HT; ++h) {
+      uint2 raw[NC];
+      uint32_t top = 0;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        raw[c] = h * 8 + g < G ? *reinterpret_cast<const uint2*>(q + (size_t)(h * 8 + g) * D + c * 16 + 4 * j) : make_uint2(0u, 0u);
+        top = max(top, kv8::top_of(make_uint4(raw[c].x, raw[c].y, 0u, 0u)));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // the largest element lies in [1, 2) after the division (a subnormal top: as it is, times 2^120)
+      const int e = max(-120, min(120, (int)(top >> 7) - 127));
+      const float inv = kv8::power_of_two(-e);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        qf[h][c][0] = pack_f16(kv8::lo_f32(raw[c].x) * inv, kv8::hi_f32(raw[c].x) * inv);
+        qf[h][c][1] = pack_f16(kv8::lo_f32(raw[c].y) * inv, kv8::hi_f32(raw[c].y) * inv);
+      }
+      const float mine = kv8::power_of_two(e);
+      f[h][0] = __shfl_sync(0xffffffffu, mine, 8 * j);
+      f[h][1] = __shfl_sync(0xffffffffu, mine, 8 * j + 4);
+    }
+    float m[HT][2], l[HT][2], o[HT][NC][4];
+#pragma unroll
+    for (int h = 0; h < HT; ++h) {
+      m[h][0] = m[h][1] = -1e30f;
+      l[h][0] = l[h][1] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) o[h][c][0] = o[h][c][1] = o[h][c][2] = o[h][c][3] = 0.f;
+    }
+    // Scores s (S^T fragment of 16 positions from position `first` on) -> p in place, its sums, the reference raised where needed.
+    // `k_unit`: what a unit of s is worth beside q's power; `ev`: log2 of the value scale, `v_inv` = 2^-ev.
+    auto softmax = [&](float (&s)[HT][4], int first, bool ragged, float k_unit, float ev, float v_inv) {
+      bool in0 = true, in1 = true;
+      if (ragged) {
+        const int p0 = first + g, p1 = p0 + 8;
+        in0 = (p0 >= lo || p0 < keep) && p0 <= pos;
+        in1 = (p1 >= lo || p1 < keep) && p1 <= pos;
+      }
+      bool grow = false;
+      float mx[HT][2];
+#pragma unroll
+      for (int h = 0; h < HT; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float unit = f[h][e] * k_unit;
+          float a = s[h][e], b = s[h][e + 2];
+          if (p.cap_out > 0.f) {
+            a = fmaf(tanhf(a * (unit * p.cap_in)), p.cap_out, ev);
+            b = fmaf(tanhf(b * (unit * p.cap_in)), p.cap_out, ev);
+          } else {
+            a = fmaf(a, unit * p.scale_log2, ev);
+            b = fmaf(b, unit * p.scale_log2, ev);
+          }
+          a = in0 ? a : -INFINITY;
+          b = in1 ? b : -INFINITY;
+          s[h][e] = a;
+          s[h][e + 2] = b;
+          float x = fmaxf(a, b);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          mx[h][e] = x;
+          grow |= x > m[h][e] + kSlack;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int h = 0; h < HT; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float now = fmaxf(m[h][e], mx[h][e]), by = ex2(m[h][e] - now);
+            m[h][e] = now;
+            l[h][e] *= by;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) { o[h][c][e] *= by; o[h][c][e + 2] *= by; }
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < HT; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[h][e] = ex2(s[h][e] - (m[h][e] - kLift));
+          s[h][e + 2] = ex2(s[h][e + 2] - (m[h][e] - kLift));
+          l[h][e] = fmaf(s[h][e] + s[h][e + 2], v_inv, l[h][e]);
+        }
+    };
+
+    if (has_tail) {
+      // the own block, in bfloat16: 16 positions per warp, from memory
+      const int first = own * PAGE + key0;
+      const bool any = first <= pos && (first + 15 >= lo || first < keep);
+      if (any) {
+        const size_t tail = ((size_t)slot * p.n_kv_heads + kvh) * (PAGE * D);
+        const __nv_bfloat16 *kt = p.k_tail + tail + key0 * D, *vt = p.v_tail + tail + key0 * D;
+        float s[HT][4] = {};
+#pragma unroll
+        for (int c = 0; c < NC; c += 2) {
+          // a lane's 16 bytes of a row fill its places in two steps of k
+          const uint4 x = *reinterpret_cast<const uint4*>(kt + g * D + c * 16 + 8 * j);
+          const uint4 y = *reinterpret_cast<const uint4*>(kt + (g + 8) * D + c * 16 + 8 * j);
+          const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+#pragma unroll
+          for (int h = 0; h < HT; ++h) {
+            const uint4 b = h * 8 + g < G ? *reinterpret_cast<const uint4*>(q + (size_t)(h * 8 + g) * D + c * 16 + 8 * j)
+                                          : make_uint4(0u, 0u, 0u, 0u);
+            mma_bf16(s[h], a0, b.x, b.y);
+            mma_bf16(s[h], a1, b.z, b.w);
+          }
+        }
+        // (these queries are whole: undo q's power)
+        float keep_f[HT][2];
+#pragma unroll
+        for (int h = 0; h < HT; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) { keep_f[h][e] = f[h][e]; f[h][e] = 1.f; }
+        softmax(s, first, true, 1.f, 0.f, 1.f);
+#pragma unroll
+        for (int h = 0; h < HT; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) f[h][e] = keep_f[h][e];
+        uint32_t b[HT][2];
+#pragma unroll
+        for (int h = 0; h < HT; ++h) {
+          b[h][0] = transposed(pack_bf16(s[h][0], s[h][1]));
+          b[h][1] = transposed(pack_bf16(s[h][2], s[h][3]));
+        }
+        bool in[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int kp = first + 2 * j + (r & 1) + (r >> 1) * 8;
+          in[r] = (kp >= lo || kp < keep) && kp <= pos;
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            w[r] = in[r] ? *reinterpret_cast<const uint32_t*>(vt + (2 * j + (r & 1) + (r >> 1) * 8) * D + c * 16 + 2 * g) : 0u;
+          const uint32_t a[4] = {__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x5410),
+                                 __byte_perm(w[2], w[3], 0x7632)};
+#pragma unroll
+          for (int h = 0; h < HT; ++h) mma_bf16(o[h][c], a, b[h][0], b[h][1]);
+        }
+      }
+    }
+
+    const uint32_t ring_u = smem_u32(ring);
+    float ks_all = 0.f, vs_all = 0.f;
+    for (int i = begin; i < end; ++i) {
+      const int n = i - begin, st = n % STAGES;
+      if ((n & 31) == 0) {                                  // scales of the next 32 items, one per lane
+        const int at = i + lane;
+        int page = at < end ? table[block_of(at)] : -1;
+        const bool ok = page >= 0 && page < total_pages;
+        ks_all = ok ? p.k_scale[(size_t)page * p.n_kv_heads + kvh] : 0.f;
+        vs_all = ok ? p.v_scale[(size_t)page * p.n_kv_heads + kvh] : 1.f;
+      }
+      const float ks = __shfl_sync(0xffffffffu, ks_all, n & 31), vs = __shfl_sync(0xffffffffu, vs_all, n & 31);
+      const int ev_i = (int)((__float_as_uint(vs) >> 23) & 0xffu) - 127;                  // vs = 2^ev_i
+      if (!mbar_wait(&full_bar[st], (n / STAGES) & 1, aborted)) break;
+      __syncwarp();
+      const int first = block_of(i) * PAGE + key0;
+      const bool ragged = first < lo && first + 15 >= keep;                 // (every position of a complete block is before pos)
+      const uint32_t kt = ring_u + st * 2 * S::TILE, vt = kt + S::TILE;
+      if (ragged) {
+        // value rows that the query does not see become zeros (e4m3 may hold a NaN there): two lanes a row
+        const int row = key0 + (lane >> 1), kp = block_of(i) * PAGE + row;
+        if (kp < lo && kp >= keep) {
+#pragma unroll
+          for (int c = 0; c < NC / 2; ++c)
+            *reinterpret_cast<uint4*>(ring + st * 2 * S::TILE + S::TILE + chunk_at<D>(row, (lane & 1) * (NC / 2) + c)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+      }
+      float s[HT][4] = {};
+#pragma unroll
+      for (int c = 0; c < NC; c += 2) {
+        uint32_t w[4];                                      // positions 0-7 and 8-15 of chunk c, then of chunk c + 1
+        ldmatrix_x4(w, kt + chunk_at<D>(key0 + (lane & 15), c + (lane >> 4)));
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t a[4];
+          numbers<FMT, false>(w[2 * u], a[0], a[2]);
+          numbers<FMT, false>(w[2 * u + 1], a[1], a[3]);
+#pragma unroll
+          for (int h = 0; h < HT; ++h) mma_f16(s[h], a, qf[h][c + u][0], qf[h][c + u][1]);
+        }
+      }
+      softmax(s, first, ragged, ks, (float)ev_i, kv8::power_of_two(-ev_i));
+      uint32_t b[HT][2];
+#pragma unroll
+      for (int h = 0; h < HT; ++h) {
+        b[h][0] = transposed(pack_f16(s[h][0], s[h][1]));
+        b[h][1] = transposed(pack_f16(s[h][2], s[h][3]));
+      }
+#pragma unroll
+      for (int c = 0; c < NC; c += 2) {
+        uint32_t w[4];
+        ldmatrix_x4_trans(w, vt + chunk_at<D>(key0 + (lane & 15), c + (lane >> 4)));
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t a[4];
+          numbers<FMT, true>(w[2 * u], a[0], a[1]);
+          numbers<FMT, true>(w[2 * u + 1], a[2], a[3]);
+#pragma unroll
+          for (int h = 0; h < HT; ++h) mma_f16(o[h][c + u], a, b[h][0], b[h][1]);
+        }
+      }
+      // the zeros written above must be ordered before the copy engine writes this stage again
+      if (ragged) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty_bar[st]);
+    }
+    // l is a sum over this lane's positions: complete it over the lanes with the same heads
+#pragma unroll
+    for (int h = 0; h < HT; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], 4);
+        l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], 8);
+        l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], 16);
+      }
+    // every warp is done with the ring; all of them go on, or none (whatever the producer sets meanwhile)
+    if (!any_consumer(*aborted != 0)) {
+      float* mo = reinterpret_cast<float*>(ring);           // [warps][heads][D]
+#pragma unroll
+      for (int h = 0; h < HT; ++h) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<float2*>(mo + ((size_t)(warp * HT + h) * 8 + 2 * j + e) * D + c * 16 + 2 * g) = make_float2(o[h][c][e], o[h][c][e + 2]);
+        if (g == 0)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) { wm[warp][h * 8 + 2 * j + e] = m[h][e]; wl[warp][h * 8 + 2 * j + e] = l[h][e]; }
+      }
+      consumers_sync();
+      for (int idx = tid; idx < G * D; idx += 32 * CONSUMERS) {
+        const int h = idx / D, d = idx % D, head = kvh * G + h;
+        float M = -1e30f, L = 0.f, acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < CONSUMERS; ++w) M = fmaxf(M, wm[w][h]);
+#pragma unroll
+        for (int w = 0; w < CONSUMERS; ++w) {
+          const float by = exp2f(wm[w][h] - M);
+          L += by * wl[w][h];
+          acc += by * mo[(size_t)(w * HT * 8 + h) * D + d];
+        }
+        if (p.n_splits == 1) {
+          L += sink_term(p.sink, head, M);
+          p.out[((size_t)t * p.n_heads + head) * D + d] = __float2bfloat16_rn(L == 0.f ? 0.f : acc / L);
+        } else {
+          const size_t at = ((size_t)t * p.n_heads + head) * p.n_splits + split;
+          p.part_o[at * D + d] = acc;
+          if (d == 0) p.part_ml[at] = make_float2(M, L);
+        }
+      }
+      if (has_tail && pos % PAGE == PAGE - 1) {
+        // the block is complete: its codes and scales, for later steps
+        const int page = table[own];
+        if (page >= 0 && page < total_pages) {
+          const size_t tail = ((size_t)slot * p.n_kv_heads + kvh) * (PAGE * D), tile = ((size_t)page * p.n_kv_heads + kvh) * (PAGE * D);
+          constexpr int PER = PAGE * D / 8 / (32 * CONSUMERS);
+#pragma unroll 1
+          for (int which = 0; which < 2; ++which) {
+            const uint4* src = reinterpret_cast<const uint4*>((which ? p.v_tail : p.k_tail) + tail);
+            uint4 v[PER];
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) { v[i] = src[tid + i * 32 * CONSUMERS]; top = max(top, kv8::top_of(v[i])); }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) top_s[which][warp] = top;
+            consumers_sync();
+#pragma unroll
+            for (int w = 0; w < CONSUMERS; ++w) top = max(top, top_s[which][w]);
+            const int e = kv8::scale_exponent<FMT>(__uint_as_float(top << 16));
+            const float inv = kv8::power_of_two(-e);
+            uint2* dst = reinterpret_cast<uint2*>((which ? p.v : p.k) + tile);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) dst[tid + i * 32 * CONSUMERS] = kv8::codes8<FMT>(v[i], inv);
+            if (tid == 0) (which ? p.v_scale_w : p.k_scale_w)[(size_t)page * p.n_kv_heads + kvh] = kv8::power_of_two(e);
+          }
+        } else if (tid == 0 && p.error_flag) {
+          atomicExch(p.error_flag, 3);
+        }
+      }
+    }
+  }
+  if (*aborted) {
+    // a wait ran out: say so, give the copies in flight time to land before the shared memory is released
+    if (lane == 0 && p.error_flag) atomicExch(p.error_flag, 1);
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  }
+}
+
+// out[t, h] = sum_s w_s O_s / sum_s w_s L_s, w_s = 2^(m_s - max m): a block per (token, head), a thread per feature.
+template <int D>
+__global__ void __launch_bounds__(D) attention_decode_kv8_combine(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
+                                                                  __nv_bfloat16* __restrict__ out, int n_splits, const float* __restrict__ sink,
+                                                                  int n_heads) {
+  __shared__ float w_s[kMaxSplits];
+  __shared__ float red[D / 32];
+  const int tid = threadIdx.x;
+  const size_t th = blockIdx.x;
+  const float2* ml = part_ml + th * n_splits;
+  const float* po = part_o + th * n_splits * D;
+  pdl_wait();
+  pdl_launch_dependents();
+  float M = -1e30f, L = 0.f, acc = 0.f;
+  if (n_splits <= 16) {
+    // every thread takes all pairs and its own feature of every part at once: one trip to the L2, no barrier
+    float2 a[16];
+    float v[16];
+#pragma unroll
+    for (int s = 0; s < 16; ++s) {
+      a[s] = s < n_splits ? __ldcg(ml + s) : make_float2(-1e30f, 0.f);
+      v[s] = s < n_splits ? __ldcg(po + (size_t)s * D + tid) : 0.f;
+    }
+#pragma unroll
+    for (int s = 0; s < 16; ++s) M = fmaxf(M, a[s].x);
+#pragma unroll
+    for (int s = 0; s < 16; ++s) {
+      const float by = exp2f(a[s].x - M);
+      L += by * a[s].y;
+      acc += by * v[s];
+    }
+  } else {
+    for (int s = tid; s < n_splits; s += D) M = fmaxf(M, __ldcg(ml + s).x);
+    M = warp_max(M);
+    if ((tid & 31) == 0) red[tid >> 5] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) M = fmaxf(M, red[w]);
+    __syncthreads();
+    for (int s = tid; s < n_splits; s += D) {
+      const float2 a = __ldcg(ml + s);
+      const float by = exp2f(a.x - M);
+      w_s[s] = by;
+      L += by * a.y;
+    }
+    L = block_sum(L, red);                                  // (its barriers also publish w_s)
+    for (int s0 = 0; s0 < n_splits; s0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = s0 + i < n_splits ? __ldcg(po + (size_t)(s0 + i) * D + tid) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (s0 + i < n_splits) acc += w_s[s0 + i] * v[i];
+    }
+  }
+  L += sink_term(sink, (int)(th % n_heads), M);
+  out[th * D + tid] = __float2bfloat16_rn(L == 0.f ? 0.f : acc / L);
+}
+
+template <int D, int FMT, int HT>
+int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int n_tokens, cudaStream_t stream) {
+  auto* kernel = attention_decode_kv8_kernel<D, FMT, HT>;
+  constexpr int MERGE = CONSUMERS * HT * 8 * D * 4;
+  constexpr int SMEM = (Shape<D>::RING > MERGE ? Shape<D>::RING : MERGE) + 1024;
+  static bool ready[64] = {};                               // per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !ready[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess) {
+      cudaGetLastError();
+      set_error("attention_decode_kv8: cannot reserve %d bytes of shared memory", SMEM);
+      return 1;
+    }
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  cpi::launch_pdl(kernel, dim3(p.n_splits, p.n_kv_heads, n_tokens), NT, SMEM, stream, mk, mv, p);
+  if (check_launch("attention_decode_kv8")) return 2;
+  if (p.n_splits > 1) {
+    cpi::launch_pdl(attention_decode_kv8_combine<D>, n_tokens * p.n_heads, D, 0, stream, p.part_o, p.part_ml, p.out, p.n_splits, p.sink,
+                    p.n_heads);
+    return check_launch("attention_decode_kv8_combine");
+  }
+  return 0;
+}
+
+}  // namespace dec8
+}  // namespace cpi
+
+using namespace cpi;
+
+extern "C" int cpi_attention_decode_kv8_supported(int n_heads, int n_kv_heads, int head_dim, int page_size) {
+  if (n_kv_heads <= 0 || n_heads % n_kv_heads) return 0;
+  return (head_dim == 64 || head_dim == 128) && page_size == kv8::PAGE && n_heads / n_kv_heads <= 16 && n_kv_heads <= 65535;
+}
+
+// Blocks of threads that share an SM, for the caller's choice of `n_splits`.
+extern "C" int cpi_attention_decode_kv8_blocks_per_sm(int group) { return group <= 8 ? 3 : 2; }
+
+// q, out [T, NH, D] bfloat16, one token per sequence; codes k, v [n_pages, NKV, 64, D]; `fmt` 0 int8, 1 e4m3.  `scratch`:
+// T * NH * splits * (D + 2) floats, 8-byte aligned (unused when n_splits == 1).
+extern "C" int cpi_attention_decode_kv8(const void* q, void* out, void* k, void* v, float* k_scale, float* v_scale, int n_pages,
+                                        const void* k_tail, const void* v_tail, int n_slots, const int* page_table, int max_blocks,
+                                        const int* token_seq, const int* token_pos, const int* seq_slot, int n_seqs, int n_tokens, int n_heads,
+                                        int n_kv_heads, int head_dim, int fmt, int window_kind, int window_size, int keep_first, float scale,
+                                        float softcap, const float* sink, int n_splits, float* scratch, int* error_flag, cudaStream_t stream) {
+  if (n_tokens == 0) return 0;
+  CPI_REQUIRE(cpi_attention_decode_kv8_supported(n_heads, n_kv_heads, head_dim, kv8::PAGE),
+              "attention_decode_kv8: unsupported shape (heads %d/%d, head size %d)", n_heads, n_kv_heads, head_dim);
+  CPI_REQUIRE(fmt == kv8::kInt8 || fmt == kv8::kE4m3, "attention_decode_kv8: unknown format %d", fmt);
+  CPI_REQUIRE(window_kind == 0 || window_size > 0, "attention_decode_kv8: window kind %d needs a size > 0", window_kind);
+  CPI_REQUIRE(n_splits >= 1 && n_splits <= dec8::kMaxSplits && n_tokens <= 65535, "attention_decode_kv8: bad grid (%d splits of at most %d, %d tokens)",
+              n_splits, dec8::kMaxSplits, n_tokens);
+  CPI_REQUIRE(n_splits == 1 || scratch, "attention_decode_kv8: split scratch is missing");
+  // the codes as lines of 128 bytes: a (page, head) tile is 64 * D / 128 of them
+  CUtensorMap mk, mv;
+  const uint64_t lines = (uint64_t)n_pages * n_kv_heads * (kv8::PAGE * head_dim / 128);
+  CPI_REQUIRE(n_pages > 0 && lines + kv8::PAGE < (1ull << 31), "attention_decode_kv8: a cache of %d pages of %d heads", n_pages, n_kv_heads);
+  if (tc::get_map_2d_bf16(k, 64, lines, 128, 64, kv8::PAGE * head_dim / 128, &mk)) return 1;
+  if (tc::get_map_2d_bf16(v, 64, lines, 128, 64, kv8::PAGE * head_dim / 128, &mv)) return 1;
+  const long parts = (long)n_tokens * n_heads * n_splits;
+  dec8::Params p{(const __nv_bfloat16*)q, (__nv_bfloat16*)out, k_scale, v_scale, (const __nv_bfloat16*)k_tail, (const __nv_bfloat16*)v_tail,
+                 (uint8_t*)k, (uint8_t*)v, k_scale, v_scale, page_table, max_blocks, n_pages, n_slots, n_seqs, token_seq, token_pos, seq_slot,
+                 n_heads, n_kv_heads, window_kind, window_size, keep_first > 0 ? keep_first : 0, scale * 1.4426950408889634f,
+                 softcap > 0.f ? scale / softcap : 0.f, softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, n_splits,
+                 scratch, scratch ? reinterpret_cast<float2*>(scratch + parts * head_dim) : nullptr, sink, error_flag};
+  const bool wide = n_heads / n_kv_heads > 8;
+#define CPI_DEC8(D, F) (wide ? dec8::launch<D, F, 2>(mk, mv, p, n_tokens, stream) : dec8::launch<D, F, 1>(mk, mv, p, n_tokens, stream))
+  if (head_dim == 128) return fmt ? CPI_DEC8(128, 1) : CPI_DEC8(128, 0);
+  return fmt ? CPI_DEC8(64, 1) : CPI_DEC8(64, 0);
+#undef CPI_DEC8
+}

@@ -28,6 +28,14 @@
 // and 4,096 tokens 324 (530 TFLOP/s).  The cap compiled apart, a row's mask as one word per 32 columns and a small loop for the
 // first tile's maximum: 8.4, 138 and 226 us (760; 961 at 16,384 tokens).
 //
+// BLOCKED: attention over the cache in 8 bits (kv8.cuh).  A query sees its own block of 64 positions as projected and earlier
+// blocks as the numbers they are held as; both stand in bfloat16 pages of the step's own, named by two tables.  The axis of key
+// tiles then begins with the exact tiles of query tile A, goes on with the earlier blocks' and ends with the exact tiles of B: A
+// meets a prefix of it and B a suffix, as without BLOCKED.  A row's mask is that of the window cut at the start of its block,
+// from one side or the other.  Pages that a tile does not have are asked for beyond the tensor's end and arrive as zeros, rows
+// behind the newest position are zero already: nothing is overwritten in shared memory.  Per query tile that is one or two key
+// tiles more than without (they hold the own blocks twice).
+//
 // Every mbarrier wait is bounded; when one runs out the CTA sets *error_flag and leaves.
 #include "prefill_tc.cuh"
 #include <type_traits>
@@ -49,12 +57,14 @@ struct Params {
   const float* sink;                  // [NH] float32 or null: exp(sink[h]) joins the softmax denominator (no key, no value)
   int keep_first;                     // sliding window: a sequence's first positions stay visible to every later query
   float cap_in, cap_out;              // soft cap c > 0 on the scaled scores: cap_in = scale / c, cap_out = c log2(e); else 0
+  const int* exact_table;             // BLOCKED: pages by sequence of the step and block (page_table: those of earlier blocks), -1 none
+  int n_pages;
 };
 
 
 constexpr int kRingSlots = 5;           // key and value tiles in shared memory at a time
 
-template <int D, bool CAPPED>
+template <int D, bool CAPPED, bool BLOCKED = false>
 __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                 const __grid_constant__ CUtensorMap map_k,
                                                                 const __grid_constant__ CUtensorMap map_v, Params p) {
@@ -96,7 +106,7 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
   const int tile = blockIdx.y, head = blockIdx.x;       // heads are the fast axis: all heads of the longest tile start first
   const int kvh = head / (p.n_heads / p.n_kv_heads);
   const int tok0 = p.tile_tok0[tile], rows = p.tile_rows[tile];
-  const int slot = p.seq_slot[p.token_seq[tok0]];
+  const int slot = BLOCKED ? p.token_seq[tok0] : p.seq_slot[p.token_seq[tok0]];
   // the tile's rows are consecutive positions of one sequence; rows 0-127 are query tile A, the rest tile B
   const int pos_first = p.token_pos[tok0], pos_last = pos_first + rows - 1;
   const int rows_x[2] = {min(rows, BQ), max(rows - BQ, 0)};
@@ -115,10 +125,24 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
   const int keep = p.window_kind == 2 ? p.keep_first : 0;
   const int n_kept = min((keep + BKV - 1) / BKV, kb_phys[0]);
   const int gap = kb_phys[0] - n_kept;
-  const int kb_x[2] = {0, has_b && keep == 0 ? kb_phys[1] - gap : 0};
-  const int ke_x[2] = {p1_x[0] / BKV + 1 - gap, has_b ? p1_x[1] / BKV + 1 - gap : 0};
+  // BLOCKED: exact tiles of A, then earlier blocks' tiles up to the one that holds the last position before A's (B's) last
+  // row's block, then exact tiles of B
+  const int first_exact[2] = {p0_x[0] / BKV, p0_x[1] / BKV};
+  const int n_exact[2] = {BLOCKED ? p1_x[0] / BKV - first_exact[0] + 1 : 0, BLOCKED && has_b ? p1_x[1] / BKV - first_exact[1] + 1 : 0};
+  auto tiles_to = [&](int x) { return BLOCKED ? max((p1_x[x] / PAGE * PAGE + BKV - 1) / BKV - gap, 0) : p1_x[x] / BKV + 1 - gap; };
+  const int n_earlier = tiles_to(has_b ? 1 : 0);
+  const int kb_x[2] = {0, n_exact[0] + (has_b && keep == 0 ? kb_phys[1] - gap : 0)};
+  const int ke_x[2] = {n_exact[0] + tiles_to(0), has_b ? n_exact[0] + n_earlier + n_exact[1] : 0};
   const int kt0 = 0, kt1 = has_b ? ke_x[1] : ke_x[0];                     // the union: every tile in it is met by A or B
-  auto key_tile = [&](int kt) { return kt < n_kept ? kt : kt + gap; };
+  auto is_exact = [&](int kt) { return BLOCKED && (kt < n_exact[0] || kt >= n_exact[0] + n_earlier); };
+  auto key_tile = [&](int kt) {
+    if (BLOCKED) {
+      if (kt < n_exact[0]) return first_exact[0] + kt;
+      kt -= n_exact[0];
+      if (kt >= n_earlier) return first_exact[1] + kt - n_earlier;
+    }
+    return kt < n_kept ? kt : kt + gap;
+  };
   const uint32_t tmem_s = tmem_base_s, tmem_o = tmem_base_s + 256;        // + 128 for tile B, both
   volatile int* abort_flag = &abort_s;
   bool ok = true;
@@ -135,14 +159,22 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
       int n = 0;                                         // item of the ring: 2 (kt - kt0) for keys, + 1 for values
       for (int kt = kt0; kt < kt1 && ok; ++kt) {
         const int blk0 = key_tile(kt) * (BKV / PAGE);
-        const int n_pages = min(BKV / PAGE, last_block - blk0 + 1);
+        const int n_pages = BLOCKED ? BKV / PAGE : min(BKV / PAGE, last_block - blk0 + 1);
+        const int* pages = BLOCKED && is_exact(kt) ? p.exact_table + (size_t)slot * p.max_blocks : table;
         const uint32_t bytes = (uint32_t)n_pages * HALVES * (PAGE * 128);
         for (int which = 0; which < 2; ++which, ++n) {
           const int s = n % NSLOT;
           if (n >= NSLOT && !mbar_wait(&kv_empty[s], ((n / NSLOT) - 1) & 1, abort_flag)) { ok = false; break; }
           mbar_expect_tx(&kv_full[s], bytes);
           for (int pg = 0; pg < n_pages; ++pg) {
-            const int row = (table[blk0 + pg] * p.n_kv_heads + kvh) * PAGE;
+            int page = 0;
+            if (BLOCKED) {                               // a page that the step does not have: beyond the tensor, zeros
+              page = blk0 + pg < p.max_blocks ? pages[blk0 + pg] : -1;
+              if (page < 0 || page >= p.n_pages) page = p.n_pages;
+            } else {
+              page = table[blk0 + pg];
+            }
+            const int row = (page * p.n_kv_heads + kvh) * PAGE;
             for (int h = 0; h < HALVES; ++h)
               tma_load_2d(ring + s * KV_BYTES + h * HALF_BYTES + pg * (PAGE * 128), which ? &map_v : &map_k,
                           &kv_full[s], h * 64, row);
@@ -252,7 +284,9 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
     const float sc = CAPPED ? p.cap_out : p.scale_log2, cap_in = p.cap_in;
     // the union's last key tile holds positions beyond the newest one: their value rows are zeroed by the group
     // whose P V on that tile is issued first (A if it meets the tile, otherwise B)
-    const bool zero_duty = x == 0 ? (kt1 - 1 >= kb_x[0] && kt1 - 1 < ke_x[0]) : !(kt1 - 1 >= kb_x[0] && kt1 - 1 < ke_x[0]);
+    const int edge = BLOCKED && live ? qp / PAGE * PAGE : 0;        // the row's own block begins here
+    const int edge_first = p0_x[x] / PAGE * PAGE;
+    const bool zero_duty = BLOCKED ? false : x == 0 ? (kt1 - 1 >= kb_x[0] && kt1 - 1 < ke_x[0]) : !(kt1 - 1 >= kb_x[0] && kt1 - 1 < ke_x[0]);
     int j = 0;
     bool okl = rows_x[x] > 0;
     for (int kt = kb_x[x]; kt < ke_x[x] && okl; ++kt, ++j) {
@@ -276,7 +310,18 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
       if (!okl) break;
       fence_after_sync();
       // a tile that lies wholly inside every row's window needs no position tests
-      const bool no_mask = key0 + BKV - 1 <= p0_x[x] && (key0 >= lo_last || key0 + BKV - 1 < keep);
+      const bool exact = is_exact(kt);
+      const bool no_mask = (BLOCKED ? !exact && key0 + BKV <= edge_first : key0 + BKV - 1 <= p0_x[x]) &&
+                           (key0 >= lo_last || key0 + BKV - 1 < keep);
+      auto sees = [&](int first) {
+        uint32_t in = visible(qp, lo, keep, first);
+        if (BLOCKED) {
+          const int n = edge - first;
+          const uint32_t before = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+          in &= exact ? ~before : before;
+        }
+        return in;
+      };
       // One pass over the row's 128 columns of S, 32 at a time with the next chunk's load in flight: the
       // maximum, P = 2^(s c - ref) as packed bf16, and the sum.  P is kept in registers until the pass is
       // known to stand, because it goes over the S it came from.
@@ -290,7 +335,7 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
         for (int c = 0; c < BKV; c += 32) {
           float v[32], mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           tmem_ld32(s_row + c, v);
-          const uint32_t in = visible(qp, lo, keep, key0 + c);
+          const uint32_t in = sees(key0 + c);
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             if (CAPPED) v[e] = tanh_fast(v[e] * cap_in);
@@ -319,7 +364,7 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
               v[e] = exp2_fast(fmaf(sv, sc, nref));
             }
           } else {
-            const uint32_t in = visible(qp, lo, keep, key0 + cc * 32);
+            const uint32_t in = sees(key0 + cc * 32);
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               float sv = __uint_as_float(raw[cc & 1][e]);
@@ -439,7 +484,7 @@ extern "C" int cpi_attention_prefill(const void* q, void* out, const void* k_cac
   pre::Params p{(__nv_bfloat16*)out, page_table, max_blocks, token_pos, token_seq, seq_slot, tile_tok0, tile_rows,
                 n_heads, n_kv_heads, window_kind, window_size, scale * 1.4426950408889634f, error_flag, sink,
                 keep_first > 0 ? keep_first : 0, softcap > 0.f ? scale / softcap : 0.f,
-                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f};
+                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, nullptr, 0};
   dim3 grid(n_heads, n_tiles);
   const int halves = head_dim / 64;
   const int smem = halves * 128 * 128 * (2 + pre::kRingSlots);     // Q of both tiles, the ring of K and V tiles
@@ -454,4 +499,46 @@ extern "C" int cpi_attention_prefill(const void* q, void* out, const void* k_cac
   };
   if (head_dim == 128) launch_dim(std::integral_constant<int, 128>{}); else launch_dim(std::integral_constant<int, 64>{});
   return check_launch("attention_prefill");
+}
+
+// The same over the pages of a step on the cache in 8 bits: k_pages, v_pages [n_pages, NKV, 64, D] bfloat16, named per sequence of the
+// step and block by earlier_table and exact_table [sequences, width] (-1: none).
+extern "C" int cpi_attention_prefill_kv8(const void* q, void* out, const void* k_pages, const void* v_pages, long n_pages,
+                                         const int* earlier_table, const int* exact_table, int width, const int* token_seq,
+                                         const int* token_pos, const int* tile_tok0, const int* tile_rows, int n_tiles, int n_tokens,
+                                         int n_heads, int n_kv_heads, int head_dim, int window_kind, int window_size, int keep_first,
+                                         float scale, float softcap, const float* sink, int* error_flag, cudaStream_t stream) {
+  if (n_tiles == 0) return 0;
+  CPI_REQUIRE(cpi_attention_prefill_supported(n_heads, n_kv_heads, head_dim, pre::PAGE),
+              "attention_prefill_kv8: unsupported shape (heads %d/%d, head size %d)", n_heads, n_kv_heads, head_dim);
+  CPI_REQUIRE(window_kind == 0 || window_size > 0, "attention_prefill_kv8: window kind %d needs a size > 0", window_kind);
+  CPI_REQUIRE(n_tiles <= 65535, "attention_prefill_kv8: too many query tiles in one launch (%d)", n_tiles);
+  const uint64_t kv_rows = (uint64_t)n_pages * n_kv_heads * pre::PAGE;
+  CPI_REQUIRE(n_pages > 0 && kv_rows + (uint64_t)n_kv_heads * pre::PAGE < (1ull << 31), "attention_prefill_kv8: %ld pages of %d heads", n_pages, n_kv_heads);
+  CUtensorMap mq, mk, mv;
+  const uint64_t q_width = (uint64_t)n_heads * head_dim;
+  if (tc::get_map_2d_bf16(q, q_width, (uint64_t)n_tokens, q_width * 2, 64, pre::BQ, &mq)) return 1;
+  if (tc::get_map_2d_bf16(k_pages, (uint64_t)head_dim, kv_rows, (uint64_t)head_dim * 2, 64, pre::PAGE, &mk)) return 1;
+  if (tc::get_map_2d_bf16(v_pages, (uint64_t)head_dim, kv_rows, (uint64_t)head_dim * 2, 64, pre::PAGE, &mv)) return 1;
+  pre::Params p{(__nv_bfloat16*)out, earlier_table, width, token_pos, token_seq, nullptr, tile_tok0, tile_rows,
+                n_heads, n_kv_heads, window_kind, window_size, scale * 1.4426950408889634f, error_flag, sink,
+                keep_first > 0 ? keep_first : 0, softcap > 0.f ? scale / softcap : 0.f,
+                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, exact_table, (int)n_pages};
+  dim3 grid(n_heads, n_tiles);
+  const int smem = head_dim / 64 * 128 * 128 * (2 + pre::kRingSlots);
+  auto launch = [&](auto dim, auto capped) {
+    auto* kernel = pre::attention_prefill_kernel<dim.value, capped.value, true>;
+    static bool set[64] = {};                              // per device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !set[dev]) {
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (dev >= 0 && dev < 64) set[dev] = true;
+    }
+    cpi::launch_pdl(kernel, grid, pre::kThreads, smem, stream, mq, mk, mv, p);
+  };
+  auto launch_dim = [&](auto dim) {
+    if (p.cap_out > 0.f) launch(dim, std::true_type{}); else launch(dim, std::false_type{});
+  };
+  if (head_dim == 128) launch_dim(std::integral_constant<int, 128>{}); else launch_dim(std::integral_constant<int, 64>{});
+  return check_launch("attention_prefill_kv8");
 }

@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import functools
 from ctypes import c_int, c_long, c_float, c_void_p
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -25,7 +26,7 @@ MAX_DECODE_SPLITS = 256          # key splits that the combine kernel of decode 
 GENERAL_ATTENTION_MAX_DIM = 640  # largest key or value row of the general attention kernel
 PREFILL_TILE_ROWS = 256          # most query rows of one sequence that a block of the prefill attention kernel takes
 
-ABI_VERSION = 7                  # what cpi_abi_version() of a matching library answers
+ABI_VERSION = 8                  # what cpi_abi_version() of a matching library answers
 
 _lib = None
 scratch_generation = 0    # grows whenever a scratch buffer of this module is (re)allocated
@@ -1083,6 +1084,150 @@ def attention_decode(q, out, k_cache, v_cache, page_table, page_size, token_seq,
           c_float(float(softcap or 0.0)), _stream())
 
 
+# ---- the cache in 8 bits (see cpi_b200/cache/kv8.py for what it holds) ----------------------------------------------------
+def _kv8(cache, what, n_heads=None):
+    """(format, kv heads, head size) of a Kv8Cache after its checks; `n_heads`: the query heads that read it."""
+    codes = {torch.int8: 0, torch.float8_e4m3fn: 1}
+    k, v = cache.k, cache.v
+    if k.dtype not in codes or v.dtype != k.dtype or k.dim() != 4 or k.shape != v.shape:
+        raise KernelError(f"{what}: codes are int8 or float8_e4m3fn [pages, kv heads, 64, head size], keys and values alike, not "
+                          f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    pages, nkv, block, d = k.shape
+    if block != 64 or d not in (64, 128) or pages < 1 or nkv < 1:
+        raise KernelError(f"{what}: pages of 64 positions and heads of 64 or 128 elements, not {tuple(k.shape)}")
+    for t in (cache.k_scale, cache.v_scale):
+        if t.dtype != torch.float32 or t.shape != (pages, nkv):
+            raise KernelError(f"{what}: scales are float32 [{pages}, {nkv}], not {tuple(t.shape)} {t.dtype}")
+    for t in (cache.k_tail, cache.v_tail):
+        if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[1:] != (nkv, 64, d) or t.shape != cache.k_tail.shape:
+            raise KernelError(f"{what}: tails are bfloat16 [slots, {nkv}, 64, {d}], not {tuple(t.shape)} {t.dtype}")
+    for t in cache:
+        if not t.is_contiguous() or t.data_ptr() % 16:
+            raise KernelError(f"{what}: the cache's tensors are contiguous and start on 16 bytes")
+    if n_heads is not None and (n_heads < 1 or n_heads % nkv or n_heads // nkv > 16):
+        raise KernelError(f"{what}: {n_heads} query heads over {nkv} key/value heads (groups of 1 to 16)")
+    return codes[k.dtype], nkv, d
+
+
+def _on_current_device(what, *ts):
+    """Kernels are launched on the current device's stream: all of a call's tensors have to be there."""
+    _need_cuda(*ts)
+    here = torch._C._cuda_getDevice()
+    for t in ts:
+        if t is not None and t.device.index != here:
+            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{here}")
+
+
+def _i32(what, n, **ts):
+    for name, t in ts.items():
+        if t.dtype != torch.int32 or not t.is_contiguous() or (n is not None and t.numel() != n):
+            raise KernelError(f"{what}: {name} is contiguous int32" + ("" if n is None else f" [{n}]") + f", not {t.dtype} {tuple(t.shape)}")
+
+
+def _bf16_rows(what, shape, **ts):
+    for name, t in ts.items():
+        if t.dtype != torch.bfloat16 or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.data_ptr() % 16:
+            raise KernelError(f"{what}: {name} is contiguous bfloat16 {tuple(shape)} from 16 bytes on, not {t.dtype} {tuple(t.shape)}")
+
+
+def _attention_options(what, n_heads, scale, window_kind, window_size, keep_first, sink, softcap):
+    if window_kind not in (WINDOW_FULL, WINDOW_CHUNK, WINDOW_SLIDING) or (window_kind != WINDOW_FULL and window_size < 1):
+        raise KernelError(f"{what}: window kind {window_kind} of size {window_size}")
+    if keep_first < 0 or not scale > 0 or softcap is not None and softcap < 0:
+        raise KernelError(f"{what}: keep_first {keep_first}, scale {scale}, softcap {softcap}")
+    if sink is not None and (sink.dtype != torch.float32 or not sink.is_contiguous() or sink.numel() != n_heads):
+        raise KernelError(f"{what}: a sink is float32 [{n_heads}]")
+
+
+def attention_decode_kv8_supported(n_heads, n_kv_heads, head_dim, page_size) -> bool:
+    return bool(load().cpi_attention_decode_kv8_supported(c_int(n_heads), c_int(n_kv_heads), c_int(head_dim), c_int(page_size)))
+
+
+def attention_decode_kv8(q, out, cache, page_table, token_seq, token_pos, seq_slot, *, n_heads, scale, max_context,
+                         window_kind=WINDOW_FULL, window_size=0, keep_first=0, sink=None, softcap=0.0):
+    """Attention of one new token per sequence over a cache in 8 bits: q, out bfloat16 [T, n_heads * head_dim], `cache` a
+    Kv8Cache whose tails hold the new tokens' keys and values already.  A token at position p = 64 b + 63 completes its block:
+    the tail's codes and scales are written to page page_table[slot, b].  `max_context`: no sequence is longer (it sizes the
+    division of the keys over blocks of threads; any number is right, a good one is fast).  Windows, kept first positions,
+    sink and soft cap as in `attention_decode`.  A token at a negative position is a padded row: its output is zero."""
+    what = "attention_decode_kv8"
+    fmt, nkv, d = _kv8(cache, what, n_heads)
+    T = q.shape[0]
+    _on_current_device(what, q, out, *cache, page_table, token_seq, token_pos, seq_slot, sink)
+    _bf16_rows(what, (T, n_heads * d), q=q, out=out)
+    _i32(what, T, token_seq=token_seq, token_pos=token_pos)
+    _i32(what, None, seq_slot=seq_slot, page_table=page_table)
+    if page_table.dim() != 2 or T > 65535:
+        raise KernelError(f"{what}: a page table [slots, blocks] and up to 65535 tokens, not {tuple(page_table.shape)} and {T}")
+    _attention_options(what, n_heads, scale, window_kind, window_size, keep_first, sink, softcap)
+    if page_table.shape[0] < cache.k_tail.shape[0]:
+        raise KernelError(f"{what}: a page table of {page_table.shape[0]} slots, tails of {cache.k_tail.shape[0]}")
+    if T == 0:
+        return
+    longest = min(int(max_context), page_table.shape[1] * 64)
+    if window_kind != WINDOW_FULL:
+        longest = min(longest, window_size + 64 + -(-keep_first // 64) * 64)
+    splits = _kv8_splits(T * nkv, -(-max(longest, 1) // 64), n_heads // nkv)
+    scratch = None
+    if splits > 1:
+        scratch = torch.empty(T * n_heads * splits * (d + 2), dtype=torch.float32, device=q.device)
+    _call("cpi_attention_decode_kv8", _p(q), _p(out), _p(cache.k), _p(cache.v), _p(cache.k_scale), _p(cache.v_scale), c_int(cache.k.shape[0]),
+          _p(cache.k_tail), _p(cache.v_tail), c_int(cache.k_tail.shape[0]), _p(page_table), c_int(page_table.shape[1]), _p(token_seq),
+          _p(token_pos), _p(seq_slot), c_int(seq_slot.numel()), c_int(T), c_int(n_heads), c_int(nkv), c_int(d), c_int(fmt),
+          c_int(window_kind), c_int(int(window_size)), c_int(int(keep_first)), c_float(float(scale)), c_float(float(softcap or 0.0)),
+          _p(sink), c_int(splits), _p(scratch), _p(tc_error_flag(q.device)), _stream())
+
+
+def _kv8_splits(base: int, pages: int, group: int) -> int:
+    """Blocks of threads that share a sequence's keys, for `base` (token, kv head) pairs of up to `pages` pages each."""
+    slots = load().cpi_attention_decode_kv8_blocks_per_sm(c_int(group)) * sm_count()
+    want = slots // base if base <= slots else -(-4 * slots // base)
+    return max(1, min(want, (pages + 1) // 4, MAX_DECODE_SPLITS))
+
+
+def kv8_stage(cache, page_table, plan, k_pages, v_pages):
+    """The pages of a step of several tokens (`plan`: a Kv8Plan): k_pages, v_pages bfloat16 [plan.n_pages, kv heads, 64,
+    head_dim], whose exact pages hold the step's new rows already.  Fills in the rows before them from the tails and zeros
+    behind them, writes the blocks that are complete now to the cache and each sequence's open block to its tail, and puts
+    the numbers that earlier blocks stand for into the earlier pages."""
+    what = "kv8_stage"
+    fmt, nkv, d = _kv8(cache, what)
+    _on_current_device(what, *cache, page_table, plan.jobs, k_pages, v_pages)
+    _bf16_rows(what, (plan.n_pages, nkv, 64, d), k_pages=k_pages, v_pages=v_pages)
+    _i32(what, None, page_table=page_table)
+    if page_table.dim() != 2 or page_table.shape[0] < cache.k_tail.shape[0] or page_table.shape[1] < plan.width:
+        raise KernelError(f"{what}: a page table {tuple(page_table.shape)} for {cache.k_tail.shape[0]} slots and blocks up to {plan.width}")
+    _call("cpi_kv8_stage", _p(plan.jobs), c_int(plan.n_jobs), _p(page_table), c_int(page_table.shape[1]), c_int(cache.k_tail.shape[0]),
+          _p(cache.k), _p(cache.v), _p(cache.k_scale), _p(cache.v_scale), c_int(cache.k.shape[0]), _p(cache.k_tail), _p(cache.v_tail),
+          _p(k_pages), _p(v_pages), c_int(plan.n_pages), c_int(nkv), c_int(d), c_int(fmt), _p(tc_error_flag(k_pages.device)), _stream())
+
+
+def attention_prefill_kv8(q, out, k_pages, v_pages, plan, token_seq, token_pos, tile_tok0, tile_rows, *, n_heads, scale,
+                          window_kind=WINDOW_FULL, window_size=0, keep_first=0, sink=None, softcap=0.0):
+    """Attention of a step's tokens over the pages that `kv8_stage` has prepared: each query sees its own block of 64
+    positions in the exact pages and earlier ones in the earlier pages.  q, out bfloat16 [T, n_heads * head_dim]; query
+    tiles as in `attention_prefill`; the window is the plan's."""
+    what = "attention_prefill_kv8"
+    if k_pages.dim() != 4 or k_pages.shape[2] != 64 or k_pages.shape[3] not in (64, 128):
+        raise KernelError(f"{what}: pages [pages, kv heads, 64, 64 or 128], not {tuple(k_pages.shape)}")
+    nkv, d = k_pages.shape[1], k_pages.shape[3]
+    if n_heads < 1 or n_heads % nkv:
+        raise KernelError(f"{what}: {n_heads} query heads over {nkv} key/value heads")
+    _on_current_device(what, q, out, k_pages, v_pages, plan.jobs, token_seq, token_pos, tile_tok0, tile_rows, sink)
+    _bf16_rows(what, (plan.n_tokens, n_heads * d), q=q, out=out)
+    _bf16_rows(what, (plan.n_pages, nkv, 64, d), k_pages=k_pages, v_pages=v_pages)
+    _i32(what, plan.n_tokens, token_seq=token_seq, token_pos=token_pos)
+    _i32(what, tile_tok0.numel(), tile_tok0=tile_tok0, tile_rows=tile_rows)
+    _attention_options(what, n_heads, scale, window_kind, window_size, keep_first, sink, softcap)
+    names = {v: k for k, v in WINDOW_KINDS.items()}
+    if (names[window_kind], window_size if window_kind != WINDOW_FULL else 0, keep_first if window_kind == WINDOW_SLIDING else 0) != plan.window:
+        raise KernelError(f"{what}: window {names[window_kind]} of {window_size}, {keep_first} kept: the plan was made for {plan.window}")
+    _call("cpi_attention_prefill_kv8", _p(q), _p(out), _p(k_pages), _p(v_pages), c_long(plan.n_pages), _p(plan.earlier_table),
+          _p(plan.exact_table), c_int(plan.width), _p(token_seq), _p(token_pos), _p(tile_tok0), _p(tile_rows), c_int(tile_tok0.numel()),
+          c_int(plan.n_tokens), c_int(n_heads), c_int(nkv), c_int(d), c_int(window_kind), c_int(int(window_size)), c_int(int(keep_first)),
+          c_float(float(scale)), c_float(float(softcap or 0.0)), _p(sink), _p(tc_error_flag(q.device)), _stream())
+
+
 def latent_attention_supported(row: int, rank: int) -> bool:
     """Whether the tensor-core kernel of attention over cached latent rows takes rows of `row` elements whose first
     `rank` are the value."""
@@ -1315,3 +1460,38 @@ def ban_tokens(logits, ids, id_offsets):
     R, V = logits.shape
     _call("cpi_ban_tokens", _p(logits), c_long(logits.stride(0)), c_int(R), c_int(V), _p(ids), _p(id_offsets),
           _stream())
+
+
+class LogProbs(NamedTuple):
+    logprob: torch.Tensor                # float32, shaped as the targets: log p of each
+    entropy: torch.Tensor                # float32 [rows], in nats
+    top_logprobs: Optional[torch.Tensor]     # float32 [rows, top], largest first (None without `top`)
+    top_ids: Optional[torch.Tensor]          # int32 [rows, top], the lowest id first among equals
+
+
+def log_probs(logits, targets, *, top=0):
+    """Log probabilities (base e) of given tokens under the softmax of each row of logits [rows, vocab] (float32 or
+    bfloat16, any row stride), with the entropy of the row's distribution and its `top` (up to 32) most probable tokens.
+    `targets`: int32 or int64 [rows] or [rows, n]; a target below zero stands for none (0 is returned), one beyond the
+    vocabulary gives NaN.  A logit of -inf has probability zero; a row of -inf only: log probabilities -inf, entropy 0; a
+    row with NaN or +inf: NaN.  Returns new tensors."""
+    what = "log_probs"
+    if logits.dim() != 2 or logits.shape[1] < 1 or logits.stride(1) != 1 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise KernelError(f"{what}: logits are float32 or bfloat16 rows, not {logits.dtype} {tuple(logits.shape)} strides {logits.stride()}")
+    R, V = logits.shape
+    if targets.dtype not in (torch.int32, torch.int64) or targets.dim() not in (1, 2) or targets.shape[0] != R or not targets.is_contiguous():
+        raise KernelError(f"{what}: targets are contiguous int32 or int64 [{R}] or [{R}, n], not {targets.dtype} {tuple(targets.shape)}")
+    top = int(top)
+    most = int(load().cpi_log_probs_max_top())
+    if not 0 <= top <= min(most, V):
+        raise KernelError(f"{what}: top {top} of a vocabulary of {V} (at most {most})")
+    _on_current_device(what, logits, targets)
+    dev = logits.device
+    out = LogProbs(torch.empty(targets.shape, dtype=torch.float32, device=dev), torch.empty(R, dtype=torch.float32, device=dev),
+                   torch.empty((R, top), dtype=torch.float32, device=dev) if top else None,
+                   torch.empty((R, top), dtype=torch.int32, device=dev) if top else None)
+    if R:
+        _call("cpi_log_probs", _p(logits), c_int(dtype_code(logits.dtype)), c_long(logits.stride(0)), c_int(R), c_int(V), _p(targets),
+              c_int(1 if targets.dim() == 1 else targets.shape[1]), c_int(int(targets.dtype == torch.int64)), _p(out.logprob), _p(out.entropy),
+              _p(out.top_logprobs), _p(out.top_ids), c_int(top), _stream())
+    return out
