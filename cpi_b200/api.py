@@ -14,9 +14,10 @@ from typing import Callable, Optional, Sequence
 
 from .engine import Engine, GenerationRequest, GenerationResult, Generator, StepEntry
 from .sampling import SamplingParams
-from .sampling.sampler import Sampler
+from .engine.score import score_sequence
+from .sampling.sampler import Sampler, TokenScore
 
-__all__ = ["Model", "generate", "GenerationResult", "SamplingParams"]
+__all__ = ["Model", "generate", "GenerationResult", "SamplingParams", "TokenScore"]
 
 
 class Model:
@@ -38,22 +39,23 @@ class Model:
     @classmethod
     def load(cls, model_dir: str, *, dtype="bfloat16", max_batch: int = 1, max_context: int = 2048,
              max_tokens: Optional[int] = None, device="cuda:0", page_size: int = 64,
-             config_overrides: Optional[dict] = None) -> "Model":
+             config_overrides: Optional[dict] = None, cache_dtype: Optional[str] = None) -> "Model":
         """`max_batch` sequences of up to `max_context` positions each (the reference's EngineOptions
         names, include/engine/llama_engine.hpp:67-68); `max_tokens` bounds the cache instead when given.
         The cache is sized in whole pages, but generation keeps to `max_context` itself: a longer prompt
         is an error and a sequence ends when it reaches it.
         `config_overrides`: config.json keys that replace the file's, e.g. {"rope_theta": 1e6} or a
-        preset of `cpi_b200.config.registry.cli_presets()`."""
-        eng = Engine.from_model_dir(model_dir, config_overrides, dtype=dtype, device=device,
+        preset of `cpi_b200.config.registry.cli_presets()`.  `cache_dtype` "int8" or "e4m3": the attention layers'
+        keys and values are held in 8 bits, half the memory and half of what a decode step reads of them."""
+        eng = Engine.from_model_dir(model_dir, config_overrides, dtype=dtype, device=device, cache_dtype=cache_dtype,
                                     **cls._cache_args(max_batch, max_context, max_tokens, page_size))
         return cls(eng, max_batch, max_context)
 
     @classmethod
     def random(cls, config_json: dict, seed: int = 0, *, dtype="bfloat16", max_batch: int = 1,
                max_context: int = 2048, max_tokens: Optional[int] = None, device="cuda:0",
-               page_size: int = 64, config_overrides: Optional[dict] = None) -> "Model":
-        eng = Engine.from_random(config_json, seed, config_overrides, dtype=dtype, device=device,
+               page_size: int = 64, config_overrides: Optional[dict] = None, cache_dtype: Optional[str] = None) -> "Model":
+        eng = Engine.from_random(config_json, seed, config_overrides, dtype=dtype, device=device, cache_dtype=cache_dtype,
                                  **cls._cache_args(max_batch, max_context, max_tokens, page_size))
         return cls(eng, max_batch, max_context)
 
@@ -61,10 +63,12 @@ class Model:
     def generate(self, prompts: Sequence[Sequence[int]], max_new: int = 16, temperature: float = 0.8,
                  top_k: int = 40, top_p: float = 0.9, repetition_penalty: float = 1.0,
                  no_repeat_ngram_size: int = 0, seed: int = 0, stop_ids: Optional[Sequence[int]] = None,
-                 on_token: Optional[Callable[[int, int], bool]] = None) -> list:
-        """Generates for every prompt (lists of token ids); returns a GenerationResult per prompt."""
+                 on_token: Optional[Callable[[int, int], bool]] = None, logprobs: Optional[int] = None) -> list:
+        """Generates for every prompt (lists of token ids); returns a GenerationResult per prompt.  `logprobs` k: each
+        result's `scores` says of every generated token its log probability, the entropy of its distribution and the k
+        most probable tokens (up to 32), before temperature and penalties."""
         sp = SamplingParams(temperature, top_k, top_p, repetition_penalty, no_repeat_ngram_size, seed)
-        reqs = [GenerationRequest(p, max_new, sp, stop_ids) for p in prompts]
+        reqs = [GenerationRequest(p, max_new, sp, stop_ids, logprobs) for p in prompts]
         return self.generator.generate(reqs, on_token)
 
     def generate_requests(self, requests: Sequence[GenerationRequest], on_token=None) -> list:
@@ -103,12 +107,23 @@ class Model:
         finally:
             self.engine.release_slot(s)
 
+    def score(self, sequences: Sequence[Sequence[int]], top: int = 0) -> list:
+        """How probable each token of the given sequences (two tokens or more each) was after those before it: per
+        sequence of n tokens n - 1 TokenScores, of its second token to its last."""
+        out = []
+        for tokens in sequences:
+            got = score_sequence(self.engine, tokens, top)
+            lp, entropy = got.logprob.tolist(), got.entropy.tolist()
+            best = [list(zip(i, v)) for i, v in zip(got.top_ids.tolist(), got.top_logprobs.tolist())] if top else [[] for _ in lp]
+            out.append([TokenScore(*x) for x in zip(lp, entropy, best)])
+        return out
+
     def stats(self):
         return self.generator.stats
 
 
 def generate(model_dir: str, prompts, **kw) -> list:
     """One call: load `model_dir` and generate for `prompts`."""
-    load_kw = {k: kw.pop(k) for k in ("dtype", "max_context", "device") if k in kw}
+    load_kw = {k: kw.pop(k) for k in ("dtype", "max_context", "device", "cache_dtype") if k in kw}
     m = Model.load(model_dir, max_batch=max(1, len(prompts)), **load_kw)
     return m.generate(prompts, **kw)

@@ -20,6 +20,9 @@ src/engine/llama4_cuda_engine.cu:258-265).  Here:
 * **State**: a mixer may declare named tensors of fixed shape per sequence; they are kept as
   `[slots, *shape]` per run entry and zeroed when a slot is acquired.
 
+* A requirement may be **held** in 8 bits (`held`): complete blocks as codes with scales, the newest block of every
+  slot in the model's dtype (cache/kv8.py).
+
 All bookkeeping is on the host; tables are mirrored to the device before a step.
 """
 from __future__ import annotations
@@ -28,6 +31,8 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+
+from . import kv8
 
 
 class CacheError(RuntimeError):
@@ -48,6 +53,7 @@ class KVRequirement:
     window_size: int = 0
     streams: tuple = ()             # () = (("k", n_kv_heads, head_dim), ("v", n_kv_heads, head_dim))
     keep_first: int = 0             # sliding window: the sequence's first positions stay readable whatever the distance
+    held: str = ""                  # "int8" | "e4m3": keys and values of complete blocks in 8 bits (cache/kv8.py); "": the cache's dtype
 
     def stream_shapes(self) -> tuple:
         return self.streams or (("k", self.n_kv_heads, self.head_dim), ("v", self.n_kv_heads, self.head_dim))
@@ -106,11 +112,14 @@ class KVGroup:
     def __init__(self, req: KVRequirement, entries: list, n_pages: int, page_size: int, max_slots: int,
                  max_blocks: int, dtype: torch.dtype, device):
         self.req, self.entries = req, list(entries)
-        self.page_size, self.max_blocks = page_size, max_blocks
+        self.page_size, self.max_blocks, self.dtype = page_size, max_blocks, dtype
         self.pool = PagePool(n_pages)
         # zeroed once: a tensor-core kernel multiplies masked positions by zero, which needs finite values
         self.streams = {}
-        for name, heads, dim in req.stream_shapes():
+        self.kv8 = None
+        if req.held:
+            self._init_kv8(req, len(entries), n_pages, max_slots, max_blocks, dtype, device)
+        for name, heads, dim in () if req.held else req.stream_shapes():
             if name in self.streams:
                 raise CacheError(f"a cache requirement names the stream '{name}' twice")
             self.streams[name] = torch.zeros((len(entries), n_pages, int(heads), page_size, int(dim)), dtype=dtype,
@@ -122,7 +131,27 @@ class KVGroup:
         self._dirty: set = set()
         self._index = {e: i for i, e in enumerate(self.entries)}
 
+    def _init_kv8(self, req, n_entries, n_pages, max_slots, max_blocks, dtype, device) -> None:
+        if req.held not in kv8.FORMATS or req.streams or self.page_size != kv8.BLOCK or dtype != torch.bfloat16:
+            raise CacheError(f"a cache in 8 bits holds the two streams of attention in bfloat16 models, in pages of {kv8.BLOCK} positions, "
+                             f"as {' or '.join(kv8.FORMATS)}: not '{req.held}', pages of {self.page_size}, {dtype}")
+        shape = (req.n_kv_heads, kv8.BLOCK, req.head_dim)
+        code = lambda: torch.zeros((n_entries, n_pages, *shape), dtype=kv8.FORMATS[req.held], device=device)         # noqa: E731
+        scale = lambda: torch.ones((n_entries, n_pages, req.n_kv_heads), dtype=torch.float32, device=device)         # noqa: E731
+        tail = lambda: torch.zeros((n_entries, max_slots, *shape), dtype=dtype, device=device)                       # noqa: E731
+        self.kv8 = kv8.Kv8Cache(code(), code(), scale(), scale(), tail(), tail())
+        # every block of a slot is its tail page: what a kernel that stores single tokens through a page table is given
+        self.tail_table = torch.arange(max_slots, dtype=torch.int32, device=device)[:, None].expand(-1, max_blocks).contiguous()
+
+    def kv8_view(self, entry: int) -> "kv8.Kv8Cache":
+        if self.kv8 is None:
+            raise CacheError(f"run entry {entry} keeps its cache in {self.dtype}, not in 8 bits")
+        i = self._index[entry]
+        return kv8.Kv8Cache(*(t[i] for t in self.kv8))
+
     def layer_views(self, entry: int):
+        if self.kv8 is not None:
+            raise CacheError(f"run entry {entry} keeps its keys and values in 8 bits: there are no pages of them to view")
         if self.k is None or self.v is None:
             raise CacheError(f"run entry {entry} keeps the streams {sorted(self.streams)}, not keys and values")
         i = self._index[entry]
@@ -312,6 +341,11 @@ class CacheManager:
         g = self.group_of_entry[entry]
         k, v = g.layer_views(entry)
         return k, v, g.table, g.page_size
+
+    def kv8_view(self, entry: int):
+        """(Kv8Cache of run entry `entry`, page_table, tail_table): for a requirement that is held in 8 bits."""
+        g = self.group_of_entry[entry]
+        return g.kv8_view(entry), g.table, getattr(g, "tail_table", None)
 
     def stream_view(self, entry: int, name: str):
         """(tensor [pages, heads, page_size, dim], page_table, page_size) of one named stream of run entry `entry`."""

@@ -17,7 +17,8 @@ a fatal error (there is no CPU path).  --interactive speaks the reference's line
 (src/app/main_modes.cpp:46-270) with token ids in place of text: a request {"id", "tokens", "max_new",
 "temp", "stop_ids", "shutdown"}, events "start", "delta" {"tokens": [id]}, "metrics" {"token_index"},
 "done" {"tokens", "elapsed_ms", "generated_tokens", "tok_per_s"}, "error" {"error"}.
-Added here: --tokens-file, --batch-file, --stop-ids, --seed, --dtype, --random, --dump-logits, --preset and
+Added here: --tokens-file, --batch-file, --stop-ids, --seed, --dtype, --cache-dtype, --logprobs, --score, --random,
+--dump-logits, --preset and
 the options that the registered architectures declare (for instance --rope-pairing, --qk-norm-order,
 --qk-norm-scope, --router-gate); they reach the model as config.json keys.
 """
@@ -71,6 +72,11 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--stop-ids", default="", help="further stop token ids, comma separated")
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--dtype", choices=["bfloat16", "float32", "bf16", "fp32"], default="bfloat16")
+    p.add_argument("--cache-dtype", choices=["int8", "e4m3"], default=None,
+                   help="hold the attention layers' keys and values in 8 bits (default: in --dtype)")
+    p.add_argument("--logprobs", type=int, default=None, metavar="K",
+                   help="print each generated token's log probability, its distribution's entropy and the K most probable tokens")
+    p.add_argument("--score", action="store_true", help="print how probable the prompts' own tokens are, and generate nothing")
     p.add_argument("--inspect-next-topk", type=int, default=0)
     p.add_argument("--trace-steps", type=int, default=0)
     p.add_argument("--benchmark", action="store_true")
@@ -130,6 +136,10 @@ def validate(a) -> None:
         bad("--repeat-penalty must be > 0")
     if a.no_repeat_ngram < 0:
         bad("--no-repeat-ngram must be >= 0")
+    if a.logprobs is not None and not 0 <= a.logprobs <= 32:
+        bad("--logprobs must be in [0, 32]")
+    if a.cache_dtype is not None and a.dtype in ("float32", "fp32"):
+        bad("--cache-dtype goes with --dtype bfloat16")
     if a.benchmark_reps < 1 or a.benchmark_warmup < 0:
         bad("--benchmark-reps must be >= 1 and --benchmark-warmup >= 0")
 
@@ -203,7 +213,7 @@ def _main(argv=None) -> int:
             raise RuntimeError("--cpu: this library has no CPU path; the model runs on its CUDA kernels only")
         from ..api import Model
         kw = dict(dtype=a.dtype, max_batch=len(prompts), max_context=a.max_context,
-                  config_overrides=config_overrides(a))
+                  config_overrides=config_overrides(a), cache_dtype=a.cache_dtype)
         if a.random:
             with open(a.random) as f:
                 model = Model.random(json.load(f), a.seed, **kw)
@@ -219,11 +229,17 @@ def _main(argv=None) -> int:
         stops += extra_stops
         gen_kw = dict(max_new=a.max_new, temperature=a.temp, top_k=a.top_k, top_p=a.top_p,
                       repetition_penalty=a.repeat_penalty, no_repeat_ngram_size=a.no_repeat_ngram,
-                      seed=a.seed, stop_ids=stops)
+                      seed=a.seed, stop_ids=stops, logprobs=a.logprobs)
         if a.interactive:
             return interactive(model, gen_kw, sys.stdin, sys.stdout)
         print(f"[info] {spec.architecture} layers={len(spec.layers)} hidden={spec.hidden_size} "
               f"vocab={spec.vocab_size} dtype={a.dtype} prompts={len(prompts)}")
+        if a.score:
+            for i, (p, scores) in enumerate(zip(prompts, model.score(prompts, a.logprobs or 0))):
+                print_scores(p[1:], scores)
+                print(f"[score] prompt={i} tokens={len(scores)} logprob={sum(s.logprob for s in scores):.4f} "
+                      f"mean={sum(s.logprob for s in scores) / len(scores):.4f}")
+            return 0
         if a.dump_logits:
             import numpy as np
             rows = [model.next_token_logits(p).float().cpu().numpy() for p in prompts]
@@ -256,6 +272,8 @@ def _main(argv=None) -> int:
             gen += model.stats().generated_tokens
         for p, r in zip(prompts, results):
             print("Output tokens:" + "".join(f" {t}" for t in list(p) + r.tokens))
+            if r.scores is not None:
+                print_scores(r.tokens, r.scores)
         st = model.stats()
         gen, tot_ms, pre_ms, dec_ms = gen // reps, tot_ms / reps, pre_ms / reps, dec_ms / reps
         rate = lambda n, ms: 1e3 * n / ms if n > 0 and ms > 0 else 0.0
@@ -288,6 +306,11 @@ def _main(argv=None) -> int:
     except Exception as e:                                    # noqa: BLE001  (the reference: catch, print, 2)
         print(f"fatal: {type(e).__name__}: {e}", file=sys.stderr)
         return 2
+
+
+def print_scores(tokens, scores) -> None:
+    for t, s in zip(tokens, scores):
+        print(f"  id={t} logprob={s.logprob:.4f} entropy={s.entropy:.4f}" + "".join(f" {i}:{v:.4f}" for i, v in s.top))
 
 
 def interactive(model, defaults: dict, inp, out) -> int:

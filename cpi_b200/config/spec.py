@@ -11,7 +11,7 @@ run order that is itself data has no counterpart there.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Optional
 
 
@@ -26,6 +26,28 @@ class PartSpec:
 
     def get(self, key, default=None):
         return self.params.get(key, default)
+
+
+def with_cache_dtype(spec: "ModelSpec", held: str) -> "ModelSpec":
+    """The same model with the keys and values of its attention mixers held in 8 bits (`held`: "int8" or "e4m3"), those that
+    run side by side with other mixers included.  Mixers of other kinds keep what they keep."""
+    found = []
+
+    def changed(part):
+        if part.kind == "attention":
+            found.append(part)
+            return PartSpec(part.kind, {**part.params, "cache_dtype": held})
+        if part.kind == "parallel":
+            return PartSpec(part.kind, {**part.params, "branches": [{**b, "mixer": changed(b["mixer"])} for b in part.params["branches"]]})
+        return part
+
+    layers = tuple(replace(l, mixer=changed(l.mixer)) for l in spec.layers)
+    if not found:
+        raise ValueError(f"cache_dtype '{held}': no layer of this model keeps keys and values of softmax attention")
+    for i, e in enumerate(spec.run_order):
+        if e.cache_of is not None and layers[e.layer].mixer != spec.layers[e.layer].mixer:
+            raise ValueError(f"cache_dtype '{held}': run entry {i} reads entry {e.cache_of}'s cache, which 8 bits do not support")
+    return replace(spec, layers=layers)
 
 
 @dataclass(frozen=True)

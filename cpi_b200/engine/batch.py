@@ -9,12 +9,13 @@ Every array is int32 on the device, filled from one pinned host buffer with a si
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import numpy as np
 import torch
 
 
+from ..cache.kv8 import Kv8Plan
 from ..csrc.lib import PREFILL_TILE_ROWS as Q_TILE      # query rows that one block of the prefill attention kernel takes
 
 
@@ -40,6 +41,14 @@ class StepBatch:
     n_q_tiles: int = 0                 # prefill only: tiles of up to Q_TILE consecutive tokens of one sequence,
     tile_tok0: torch.Tensor = None     # first packed token of each tile, longest context first
     tile_rows: torch.Tensor = None     # tokens in each tile
+    plans: dict = field(default_factory=dict)      # prompts: by window, where the blocks lie that an 8-bit cache's layers work on
+
+    def kv8_plan(self, window_kind: str, window_size: int, keep_first: int) -> Kv8Plan:
+        key = (window_kind, window_size, keep_first)
+        if key not in self.plans:
+            self.plans[key] = Kv8Plan(self.starts, self.n_new, self.slots, window_kind=window_kind, window_size=window_size,
+                                      keep_first=keep_first, device=self.tokens.device)
+        return self.plans[key]
 
     @property
     def is_decode(self) -> bool:

@@ -16,9 +16,10 @@ from typing import Optional, Sequence
 import torch
 
 from ..cache import CacheManager
+from ..cache.kv8 import BLOCK, FORMATS
 from ..config.common import read_config_json
 from ..config.registry import apply_overrides, architecture_of, spec_from_model_dir
-from ..config.spec import ModelSpec
+from ..config.spec import ModelSpec, with_cache_dtype
 from ..csrc import lib as K
 from ..parts import Workspace
 from .. import phases
@@ -46,13 +47,22 @@ class StepEntry:
 class Engine:
     def __init__(self, spec: ModelSpec, source, *, dtype="bfloat16", device="cuda:0", max_tokens: int = 4096,
                  max_seqs: Optional[int] = None, max_seq_len: Optional[int] = None, page_size: int = 64,
-                 max_step_tokens: int = 8192, config=None):
+                 max_step_tokens: int = 8192, config=None, cache_dtype: Optional[str] = None):
+        """`cache_dtype`: "int8" or "e4m3" holds the keys and values of the attention layers in 8 bits (cache/kv8.py);
+        default: in `dtype`."""
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise RuntimeError("cpi_b200 runs on a CUDA device only; there is no CPU path")
         K.load()                                   # fails loudly when the kernel library is missing
         torch.cuda.set_device(self.device)
         self.dtype = _dtype_of(dtype)
+        self.cache_dtype = cache_dtype or None
+        if self.cache_dtype is not None:
+            if self.cache_dtype not in FORMATS:
+                raise ValueError(f"cache_dtype must be one of {sorted(FORMATS)} (or None for the model's dtype), not '{cache_dtype}'")
+            if self.dtype != torch.bfloat16 or page_size != BLOCK:
+                raise ValueError(f"cache_dtype '{cache_dtype}' goes with bfloat16 and pages of {BLOCK} positions, not {self.dtype} and {page_size}")
+            spec = with_cache_dtype(spec, self.cache_dtype)
         self.spec, self.config = spec, config
         self.ws = Workspace(self.device)
         self.model = DecoderModel(spec, self.dtype, self.device, self.ws)

@@ -27,6 +27,7 @@ class GenerationRequest:
     max_new: int = 16
     sampling: SamplingParams = GREEDY
     stop_ids: Optional[Sequence[int]] = None      # None: the model's own end tokens
+    logprobs: Optional[int] = None                # score every generated token, with that many alternatives (None: do not)
 
 
 @dataclass
@@ -34,6 +35,7 @@ class GenerationResult:
     tokens: list                                   # generated ids (the prompt is not repeated)
     finish_reason: str                             # "stop_token" | "max_new" | "capacity" | "callback"
     prompt_tokens: int
+    scores: Optional[list] = None                  # a TokenScore per generated token, if the request asked for log probabilities
 
 
 @dataclass
@@ -92,7 +94,7 @@ class Generator:
         # Decode steps are launched one ahead of the host: step n+1 takes its tokens from the device tensor
         # that the sampler of step n wrote, while the host is still reading step n's tokens for the stop
         # checks.  Needs nothing from the host between steps, so it is off for requests with a callback, a
-        # repetition penalty or n-gram bans.
+        # repetition penalty, n-gram bans or log probabilities.
         self.pipelined = True
         self._pinned = None
 
@@ -109,7 +111,9 @@ class Generator:
             if r.max_new < 1:
                 raise ValueError(f"request {i}: max_new must be >= 1")
             r.sampling.validate()
-            reqs.append(GenerationRequest(prompt, r.max_new, r.sampling, r.stop_ids))
+            if r.logprobs is not None and r.logprobs < 0:
+                raise ValueError(f"request {i}: logprobs must be a number of alternatives, 0 or more, not {r.logprobs}")
+            reqs.append(GenerationRequest(prompt, r.max_new, r.sampling, r.stop_ids, r.logprobs))
         cache = self.engine.cache
         batches = plan_batches(reqs, max_batch=self.max_batch, token_capacity=cache.n_pages * cache.page_size,
                                page_size=cache.page_size, max_seq_len=self.max_context)
@@ -125,7 +129,7 @@ class Generator:
 
     def _run_batch(self, idxs, reqs, results, on_token):
         needs_host = on_token is not None or any(
-            reqs[i].sampling.repetition_penalty > 1.0 or reqs[i].sampling.no_repeat_ngram_size > 1 for i in idxs)
+            reqs[i].logprobs is not None or reqs[i].sampling.repetition_penalty > 1.0 or reqs[i].sampling.no_repeat_ngram_size > 1 for i in idxs)
         if self.pipelined and not needs_host and hasattr(self.engine, "step_decode") \
                 and hasattr(self.sampler, "sample_device"):
             return self._run_batch_pipelined(idxs, reqs, results)
@@ -134,6 +138,7 @@ class Generator:
         live = list(idxs)
         slot = {i: eng.acquire_slot() for i in live}
         out = {i: [] for i in live}
+        scores = {i: None if reqs[i].logprobs is None else [] for i in live}
         stops = {i: set(self.default_stop_ids if reqs[i].stop_ids is None else reqs[i].stop_ids) for i in live}
         t0 = time.perf_counter()
         try:
@@ -146,7 +151,14 @@ class Generator:
                 # the histories (prompt + generated ids) are only looked at by the penalties and the n-gram bans
                 need_hist = any(p.repetition_penalty > 1.0 or p.no_repeat_ngram_size > 1 for p in params)
                 hist = [list(reqs[i].prompt) + out[i] for i in live] if need_hist else [None] * len(live)
+                asked = [reqs[i].logprobs for i in live if reqs[i].logprobs is not None]
+                # (the penalties and bans change the rows in place; the scores are of what the model said)
+                said = logits.clone() if asked and need_hist else logits
                 toks = self.sampler.sample(logits, params, hist, [(i, step) for i in live])
+                if asked:
+                    for i, s in zip(live, self.sampler.log_probs(said, toks, max(asked))):
+                        if scores[i] is not None:
+                            scores[i].append(s._replace(top=s.top[:reqs[i].logprobs]))
                 if t1 is None:                      # the first sample ends the prefill phase
                     t1 = time.perf_counter()
                     self.stats.prefill_ms += (t1 - t0) * 1e3
@@ -169,7 +181,7 @@ class Generator:
                     if reason is None:
                         nxt.append(i)
                     else:
-                        results[i] = GenerationResult(out[i], reason, len(reqs[i].prompt))
+                        results[i] = GenerationResult(out[i], reason, len(reqs[i].prompt), scores[i])
                         eng.release_slot(slot.pop(i))
                 live = nxt
                 if not live:

@@ -1,0 +1,42 @@
+"""Scores of given tokens: a sequence is run as a prompt, and every position's logits say how probable the next token was.
+
+The logits of a piece (float32 [tokens, vocab]) live in one buffer; pieces are cut so that it stays below LOGIT_BYTES.  Each
+piece's rows go through one launch of `log_probs`; nothing else of them is kept.  (The reference scores nothing: it prints the
+largest logits after a prompt, src/engine/llama4_cuda_engine.cu:623-674.)
+"""
+from __future__ import annotations
+
+from typing import Sequence
+
+import torch
+
+from ..csrc import lib as K
+from .engine import StepEntry
+
+LOGIT_BYTES = 1 << 30
+
+
+def score_sequence(engine, tokens: Sequence[int], top: int = 0) -> "K.LogProbs":
+    """Of tokens t_0 .. t_{n-1} (n >= 2) the log probabilities of t_1 .. t_{n-1} given what precedes each, the entropy of each
+    distribution and its `top` best tokens: a LogProbs of n - 1 rows on the device."""
+    tokens = [int(t) for t in tokens]
+    if len(tokens) < 2:
+        raise ValueError("a sequence to score has two tokens or more: the first is given, the others are scored")
+    n = len(tokens) - 1
+    piece = max(1, min(engine.max_step_tokens, LOGIT_BYTES // (4 * engine.spec.vocab_size)))
+    targets = torch.tensor(tokens[1:], dtype=torch.int32, device=engine.device)
+    if int(min(tokens)) < 0 or int(max(tokens)) >= engine.spec.vocab_size:
+        raise ValueError(f"a token id lies outside the vocabulary of {engine.spec.vocab_size}")
+    slot = engine.acquire_slot()
+    parts = []
+    try:
+        for a in range(0, n, piece):
+            b = min(n, a + piece)
+            logits = engine.step([StepEntry(slot, tokens[a:b], range(b - a))])
+            parts.append(K.log_probs(logits, targets[a:b], top=top))
+        engine.check_device_errors()
+    finally:
+        engine.release_slot(slot)
+    if len(parts) == 1:
+        return parts[0]
+    return K.LogProbs(*(None if c[0] is None else torch.cat(c) for c in zip(*parts)))

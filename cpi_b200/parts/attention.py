@@ -49,6 +49,10 @@ score c and no tensor: 0 adds one to the softmax denominators).  A mixer without
 temperature does its convolution (if any), rotations and cache write in one kernel (`qkv_conv_rotate`) when its sizes
 allow it.
 
+`cache_dtype` ("int8" | "e4m3"): keys and values of complete blocks of 64 positions are held in 8 bits (cache/kv8.py); a
+query sees its own block in bfloat16.  Heads of 64 or 128 elements, keys and values of one size, groups of up to 16 heads,
+one score map, no score bias.
+
 `attend(...)` below is the choice of the attention kernel for prepared queries and a paged cache; other mixers that
 end in softmax attention over pages (`latent_attention`) call it too.
 """
@@ -59,6 +63,7 @@ import math
 import numpy as np
 import torch
 
+from ..cache.kv8 import BLOCK, FORMATS
 from ..cache.manager import KVRequirement, StateRequirement
 from ..csrc import lib as K
 from ..phases import phase
@@ -139,6 +144,14 @@ class AttentionMixer(Mixer):
         limit = K.GENERAL_ATTENTION_MAX_DIM if self.general else 256
         if not 1 <= self.d <= limit or not 1 <= self.dv <= limit or (not self.general and self.d < 16):
             raise ValueError(f"attention: head sizes {self.d} / {self.dv} are not supported (up to {limit})")
+        self.cache_dtype = p.get("cache_dtype") or ""
+        if self.cache_dtype:
+            if self.cache_dtype not in FORMATS:
+                raise ValueError(f"attention: cache_dtype must be one of {sorted(FORMATS)}, not '{self.cache_dtype}'")
+            if self.d not in (64, 128) or self.dv != self.d or self.nh // self.nkv > 16 or self.maps != 1 or not self.has_kv:
+                raise ValueError(f"attention: a cache in 8 bits goes with heads of 64 or 128 elements, values of the same size, groups of up to "
+                                 f"16 heads, one score map and a cache of the layer's own, not {self.nh}/{self.nkv} heads of {self.d}/{self.dv}, "
+                                 f"{self.maps} score maps")
         self.scale = float(p["softmax_scale"])
         self.position = build_part("position", p["position"])
         self.qk_norm = bool(p.get("qk_norm", False))
@@ -285,6 +298,8 @@ class AttentionMixer(Mixer):
         if enc is not None and self.rotary is None and self.score_bias is None:
             raise TypeError(f"attention: the position part '{self.position.spec.kind}' describes itself as "
                             f"{type(enc).__name__}; this mixer's kernels take RotaryEncoding, ScoreBias or None")
+        if self.score_bias is not None and self.cache_dtype:
+            raise ValueError("attention: a cache in 8 bits does not combine with a bias on the scores")
         if self.score_bias is not None and (self.score_bias.dim() != 2 or self.score_bias.shape[0] != self.nh
                                             or self.score_bias.dtype != torch.float32):
             raise ValueError(f"attention: a score bias must be float32 [{self.nh} heads, distances], got "
@@ -298,7 +313,7 @@ class AttentionMixer(Mixer):
         if self.dv != self.d:
             return KVRequirement(self.nkv, self.d, self.window_kind, self.window_size,
                                  streams=(("k", self.nkv, self.d), ("v", self.nkv, self.dv)), keep_first=self.keep_first)
-        return KVRequirement(self.nkv, self.d, self.window_kind, self.window_size, keep_first=self.keep_first)
+        return KVRequirement(self.nkv, self.d, self.window_kind, self.window_size, keep_first=self.keep_first, held=self.cache_dtype)
 
     def state_requirements(self):
         if self.taps is None:
@@ -316,7 +331,22 @@ class AttentionMixer(Mixer):
     def forward(self, h, residual, batch, cache, add=True):
         T = h.shape[0]
         dt = h.dtype
-        k_cache, v_cache, table, page_size = cache.kv()
+        held = plan = None
+        slots = batch.seq_slot
+        if self.cache_dtype:
+            # the new rows go to the slots' tails (single tokens) or to pages of the step's own
+            held, pool_table, tail_table = cache.kv8()
+            page_size = BLOCK
+            if batch.is_decode:
+                k_cache, v_cache, table = held.k_tail, held.v_tail, tail_table
+            else:
+                plan = batch.kv8_plan(self.window_kind, self.window_size, self.keep_first)
+                shape = (plan.n_pages, self.nkv, BLOCK, self.d)
+                # (they grow with the contexts and serve this layer only: not kept between steps)
+                k_cache, v_cache = torch.empty(shape, dtype=dt, device=h.device), torch.empty(shape, dtype=dt, device=h.device)
+                table, slots = plan.exact_table, plan.seq_ids
+        else:
+            k_cache, v_cache, table, page_size = cache.kv()
         q = self.ws.get("attn_q", (T, self.nh * self.d), dt)
         if self.general:
             # float32 projection rows: bias, norm and rotation act on unrounded values
@@ -352,7 +382,7 @@ class AttentionMixer(Mixer):
                                       rotary_amplitude=amplitude)
                 else:
                     K.qkv_prepare(qkv_in, q, k_cache, v_cache, table, page_size, batch.token_seq, batch.token_pos,
-                                  batch.seq_slot, n_heads=self.nh, n_kv_heads=self.nkv, head_dim=self.d,
+                                  slots, n_heads=self.nh, n_kv_heads=self.nkv, head_dim=self.d,
                                   value_dim=self.dv, bias=self.b_qkv, q_norm=self.w_qnorm, k_norm=self.w_knorm,
                                   norm_whole=self.qk_norm and self.norm_scope == "projection",
                                   head_norm=(2 if self.norm_weight_shared else 1) if head_norm else 0,
@@ -367,15 +397,21 @@ class AttentionMixer(Mixer):
                 project(h, self.w_qkv, qkv)
             with phase("kv_store"):          # head norm, rotation, temperature and the write into the cache: one kernel
                 K.qkv_post(qkv, q, k_cache, v_cache, table, page_size, batch.token_seq, batch.token_pos,
-                           batch.seq_slot, n_heads=self.nh, n_kv_heads=self.nkv, head_dim=self.d,
+                           slots, n_heads=self.nh, n_kv_heads=self.nkv, head_dim=self.d,
                            inv_freq=None if self.rotary is None else self.rotary.inv_freq,
                            interleaved=self.rotary is not None and self.rotary.interleaved,
                            qk_norm=self.qk_norm, norm_before_rope=self.norm_before_rope,
                            norm_eps=self.qk_norm_eps, temperature=self.temperature,
                            write_kv=self.has_kv and cache.owns)
         att = self.ws.get("attn_out", (T, self.nh * self.dv), dt)
+        if plan is not None:
+            with phase("kv_store"):             # completed blocks into the cache, earlier ones into the step's pages
+                K.kv8_stage(held, pool_table, plan, k_cache, v_cache)
         with phase("attention"):
-            self.attend(q, att, k_cache, v_cache, table, page_size, batch)
+            if held is not None:
+                self.attend_kv8(q, att, held, pool_table, plan, k_cache, v_cache, batch)
+            else:
+                self.attend(q, att, k_cache, v_cache, table, page_size, batch)
             att2 = None
             if self.maps == 2:                  # the second map: its own queries and keys, the same values
                 att2 = self.ws.get("attn_out2", (T, self.nh * self.dv), dt)
@@ -398,11 +434,21 @@ class AttentionMixer(Mixer):
             project(att, self.w_o, residual, MODE_ADD if add else MODE_STORE)
 
     def _fused_preparation(self, cache) -> bool:
+        if self.cache_dtype:          # (its rows and its state go by different slots in a prompt)
+            return False
         return (use_fused_preparation and self.has_kv and cache.owns and self.maps == 1 and not self.bias and not self.qk_norm
                 and self.value_mix is None and not self.values_from_keys and self.temperature is None
                 and self.w_qkv.shape[0] % 4 == 0
                 and K.qkv_conv_rotate_supported(self.d, self.dv, self.rot_dims if self.rotary is not None else 0,
                                                 self.v_inv_freq is not None, self.taps or 1))
+
+    def attend_kv8(self, q, att, held, table, plan, k_pages, v_pages, batch):
+        how = dict(n_heads=self.nh, scale=self.scale, window_kind=K.WINDOW_KINDS[self.window_kind], window_size=self.window_size,
+                   keep_first=self.keep_first, sink=self.sink, softcap=self.softcap)
+        if plan is None:
+            K.attention_decode_kv8(q, att, held, table, batch.token_seq, batch.token_pos, batch.seq_slot, max_context=batch.ctx_bucket, **how)
+        else:
+            K.attention_prefill_kv8(q, att, k_pages, v_pages, plan, batch.token_seq, batch.token_pos, batch.tile_tok0, batch.tile_rows, **how)
 
     def attend(self, q, att, k_cache, v_cache, table, page_size, batch):
         attend(q, att, k_cache, v_cache, table, page_size, batch, n_heads=self.nh, n_kv_heads=self.nkv, head_dim=self.d,

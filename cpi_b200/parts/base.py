@@ -160,6 +160,10 @@ class CacheView:
         """(k, v, page_table, page_size): k, v are [pages, kv heads, page_size, head_dim]."""
         return self._m.kv_view(self._entry)
 
+    def kv8(self):
+        """(Kv8Cache, page_table, tail_table) of a cache that is held in 8 bits (cache/kv8.py)."""
+        return self._m.kv8_view(self._entry)
+
     def stream(self, name: str):
         """(tensor [pages, heads, page_size, dim], page_table, page_size) of a stream that the mixer's
         `KVRequirement.streams` names (attention's are "k" and "v")."""

@@ -34,6 +34,9 @@ class _BranchCache:
     def kv(self):
         return self._c.kv()
 
+    def kv8(self):
+        return self._c.kv8()
+
     def stream(self, name):
         return self._c.stream(name)
 

@@ -8,9 +8,18 @@ function of (seed, request, step), so runs repeat.
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from ..csrc import lib as K
+
+
+class TokenScore(NamedTuple):
+    """A token under the distribution that it was, or could have been, drawn from (temperature 1, no penalties)."""
+    logprob: float               # natural logarithm of the token's probability
+    entropy: float               # of the distribution, in nats
+    top: list                    # the most probable tokens as (id, log probability), largest first
 
 
 def banned_by_ngram(history: list, n: int) -> list:
@@ -85,6 +94,17 @@ class Sampler:
 
     def _f32(self, xs):
         return torch.tensor(xs, dtype=torch.float32, device=self.device)
+
+    def log_probs(self, logits: torch.Tensor, tokens, top: int = 0) -> list:
+        """What each row of logits says of the token chosen from it (waits for the device): a list of TokenScore."""
+        R = logits.shape[0]
+        targets = tokens if isinstance(tokens, torch.Tensor) else torch.tensor(tokens, dtype=torch.int32, device=logits.device)
+        got = K.log_probs(logits, targets, top=top)
+        lp, entropy = got.logprob.tolist(), got.entropy.tolist()
+        if not top:
+            return [TokenScore(lp[r], entropy[r], []) for r in range(R)]
+        ids, best = got.top_ids.tolist(), got.top_logprobs.tolist()
+        return [TokenScore(lp[r], entropy[r], list(zip(ids[r], best[r]))) for r in range(R)]
 
     def sample(self, logits: torch.Tensor, params: list, histories: list, counters: list) -> list:
         """The chosen token ids as a list (waits for the device)."""
