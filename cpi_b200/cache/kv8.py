@@ -70,11 +70,15 @@ class Kv8Plan:
         ends = [s + m for s, m in zip(starts, n_new)]
         self.width = max(-(-e // BLOCK) for e in ends)
         tables = np.full((2, n, self.width), -1, dtype=np.int32)        # [earlier, exact]
-        self.n_earlier = 0
+        self.n_earlier = self.most_tiles = 0       # most_tiles: pairs of blocks that a query tile of some sequence meets, at most
         for i, (s, m) in enumerate(zip(starts, n_new)):
             blocks = needed_blocks(s, m, *self.window)
             tables[0, i, blocks] = np.arange(self.n_earlier, self.n_earlier + len(blocks))
             self.n_earlier += len(blocks)
+            seen = len(blocks)
+            if window_kind != "full":              # a query tile's rows reach back by the window, and to the kept positions
+                seen = min(seen, -(-(window_size + 256 + self.window[2]) // BLOCK) + 2)
+            self.most_tiles = max(self.most_tiles, seen // 2 + 2)
         at = self.n_earlier
         jobs = []
         for i, (s, e) in enumerate(zip(starts, ends)):

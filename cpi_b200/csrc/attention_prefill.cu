@@ -59,6 +59,8 @@ struct Params {
   float cap_in, cap_out;              // soft cap c > 0 on the scaled scores: cap_in = scale / c, cap_out = c log2(e); else 0
   const int* exact_table;             // BLOCKED: pages by sequence of the step and block (page_table: those of earlier blocks), -1 none
   int n_pages;
+  int n_splits;                       // BLOCKED: blocks of threads that share a query tile's axis of key tiles
+  float* part_o; float2* part_ml;     // with several: [T, NH, splits, D] sums, [T, NH, splits] reference and row sum
 };
 
 
@@ -131,9 +133,16 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
   const int n_exact[2] = {BLOCKED ? p1_x[0] / BKV - first_exact[0] + 1 : 0, BLOCKED && has_b ? p1_x[1] / BKV - first_exact[1] + 1 : 0};
   auto tiles_to = [&](int x) { return BLOCKED ? max((p1_x[x] / PAGE * PAGE + BKV - 1) / BKV - gap, 0) : p1_x[x] / BKV + 1 - gap; };
   const int n_earlier = tiles_to(has_b ? 1 : 0);
-  const int kb_x[2] = {0, n_exact[0] + (has_b && keep == 0 ? kb_phys[1] - gap : 0)};
-  const int ke_x[2] = {n_exact[0] + tiles_to(0), has_b ? n_exact[0] + n_earlier + n_exact[1] : 0};
-  const int kt0 = 0, kt1 = has_b ? ke_x[1] : ke_x[0];                     // the union: every tile in it is met by A or B
+  int kb_x[2] = {0, n_exact[0] + (has_b && keep == 0 ? kb_phys[1] - gap : 0)};
+  int ke_x[2] = {n_exact[0] + tiles_to(0), has_b ? n_exact[0] + n_earlier + n_exact[1] : 0};
+  int kt0 = 0, kt1 = has_b ? ke_x[1] : ke_x[0];                           // the union: every tile in it is met by A or B
+  if (BLOCKED && p.n_splits > 1) {                                        // this block's share of the union
+    const int per = (kt1 + p.n_splits - 1) / p.n_splits;
+    kt0 = min(kt1, (int)blockIdx.z * per);
+    kt1 = min(kt1, kt0 + per);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) { kb_x[x] = min(max(kb_x[x], kt0), kt1); ke_x[x] = max(min(ke_x[x], kt1), kb_x[x]); }
+  }
   auto is_exact = [&](int kt) { return BLOCKED && (kt < n_exact[0] || kt >= n_exact[0] + n_earlier); };
   auto key_tile = [&](int kt) {
     if (BLOCKED) {
@@ -249,8 +258,9 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
       return true;
     };
     ok = __all_sync(0xffffffffu, mbar_wait(&q_full, 0, abort_flag));
-    const int kb_b = has_b ? kb_x[1] : 0x7fffffff, ke_a = ke_x[0];
-    ok = ok && issue_qk(0, kb_b != kt0);
+    // (a share of the union may have nothing for A, or nothing for B)
+    const int kb_b = has_b && (!BLOCKED || kb_x[1] < ke_x[1]) ? kb_x[1] : 0x7fffffff, ke_a = ke_x[0];
+    if (!BLOCKED || ke_a > kt0) ok = ok && issue_qk(0, kb_b != kt0);
     if (ok && kb_b == kt0) ok = issue_qk(1, true);
     for (int kt = kt0; kt < kt1 && ok; ++kt) {
       // which query tiles meet key tile kt, and kt + 1 (B's range ends with the union's, A's begins with it)
@@ -334,8 +344,9 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
 #pragma unroll 1
         for (int c = 0; c < BKV; c += 32) {
           float v[32], mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          tmem_ld32(s_row + c, v);
           const uint32_t in = sees(key0 + c);
+          if (BLOCKED && !__any_sync(0xffffffffu, in != 0)) continue;       // (no row of the warp sees a column of it)
+          tmem_ld32(s_row + c, v);
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             if (CAPPED) v[e] = tanh_fast(v[e] * cap_in);
@@ -365,6 +376,10 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
             }
           } else {
             const uint32_t in = sees(key0 + cc * 32);
+            if (BLOCKED && !__any_sync(0xffffffffu, in != 0)) {             // (no row of the warp sees a column of it)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = 0.f;
+            } else
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               float sv = __uint_as_float(raw[cc & 1][e]);
@@ -415,11 +430,27 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
     }
     // the output: O / l once the last P V is done
     ok = okl && !abort_s && j > 0;
+    if (BLOCKED && p.n_splits > 1 && live) {
+      // what this share adds up to: the row's sums and what they are measured against (nothing: a sum of zero)
+      p.part_ml[((size_t)(tok0 + x * BQ + row) * p.n_heads + head) * p.n_splits + blockIdx.z] = make_float2(m_ref, j > 0 ? l_run : 0.f);
+    }
     ok = __all_sync(0xffffffffu, ok && mbar_wait(&o_done[x], 0, abort_flag));
     fence_after_sync();
     if (ok) {
       // a sink adds 2^(sink log2 e - reference) to the row's sum and nothing to O; the exponent is capped so that a
       // sink far above every score gives a huge finite sum
+      if (BLOCKED && p.n_splits > 1) {
+        float* dst = p.part_o + (((size_t)(tok0 + x * BQ + row) * p.n_heads + head) * p.n_splits + blockIdx.z) * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float v[32];
+          tmem_ld32(o_row + c, v);
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(dst + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          }
+        }
+      } else {
       if (p.sink) l_run += exp2f(fminf(p.sink[head] * 1.4426950408889634f - m_ref, 120.f));
       const float inv = 1.0f / fmaxf(l_run, 1e-20f);
       __nv_bfloat16* dst = p.out + ((size_t)(tok0 + x * BQ + row) * p.n_heads + head) * D;
@@ -436,6 +467,7 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
           }
         }
       }
+      }
     }
     fence_before_sync();
   }
@@ -446,6 +478,41 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
   fence_before_sync();
   __syncthreads();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_s), "r"(TMEM_COLS));
+}
+
+// The shares of a query tile's keys joined: out[t, h] = sum_s w_s O_s / (sum_s w_s l_s + sink), w_s = 2^(m_s - max m).  A warp per
+// (token, head), four features or two per lane.
+template <int D>
+__global__ void __launch_bounds__(256) attention_prefill_combine(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
+                                                                 __nv_bfloat16* __restrict__ out, long rows, int n_splits,
+                                                                 const float* __restrict__ sink, int n_heads) {
+  constexpr int PER = D / 32;
+  const int lane = threadIdx.x & 31;
+  const long th = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (th >= rows) return;
+  const float2 ml = lane < n_splits ? __ldcg(part_ml + th * n_splits + lane) : make_float2(-1e30f, 0.f);
+  const float M = warp_max(ml.x);
+  const float w = exp2f(ml.x - M), l = ml.y > 0.f || ml.y != ml.y ? w * ml.y : 0.f;
+  float L = warp_sum(l), acc[PER] = {};
+  for (int s = 0; s < n_splits; ++s) {
+    const float ws = __shfl_sync(0xffffffffu, w, s), ls = __shfl_sync(0xffffffffu, ml.y, s);
+    if (ls == 0.f) continue;                             // (this share held nothing for the row, or was not written)
+    const float* src = part_o + (th * n_splits + s) * D + lane * PER;
+    if (PER == 4) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+      acc[0] += ws * v.x; acc[1] += ws * v.y; acc[PER - 2] += ws * v.z; acc[PER - 1] += ws * v.w;
+    } else {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+      acc[0] += ws * v.x; acc[1] += ws * v.y;
+    }
+  }
+  if (sink) L += exp2f(fminf(sink[th % n_heads] * 1.4426950408889634f - M, 120.f));
+  const float inv = 1.0f / fmaxf(L, 1e-20f);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(out + th * D + lane * PER);
+#pragma unroll
+  for (int i = 0; i < PER / 2; ++i) dst[i] = pack_bf16(acc[2 * i] * inv, acc[2 * i + 1] * inv);
 }
 
 }  // namespace pre
@@ -484,7 +551,7 @@ extern "C" int cpi_attention_prefill(const void* q, void* out, const void* k_cac
   pre::Params p{(__nv_bfloat16*)out, page_table, max_blocks, token_pos, token_seq, seq_slot, tile_tok0, tile_rows,
                 n_heads, n_kv_heads, window_kind, window_size, scale * 1.4426950408889634f, error_flag, sink,
                 keep_first > 0 ? keep_first : 0, softcap > 0.f ? scale / softcap : 0.f,
-                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, nullptr, 0};
+                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, nullptr, 0, 1, nullptr, nullptr};
   dim3 grid(n_heads, n_tiles);
   const int halves = head_dim / 64;
   const int smem = halves * 128 * 128 * (2 + pre::kRingSlots);     // Q of both tiles, the ring of K and V tiles
@@ -502,13 +569,17 @@ extern "C" int cpi_attention_prefill(const void* q, void* out, const void* k_cac
 }
 
 // The same over the pages of a step on the cache in 8 bits: k_pages, v_pages [n_pages, NKV, 64, D] bfloat16, named per sequence of the
-// step and block by earlier_table and exact_table [sequences, width] (-1: none).
+// step and block by earlier_table and exact_table [sequences, width] (-1: none).  `n_splits` > 1: that many blocks of threads share a query tile's
+// keys, through `scratch` (n_tokens * n_heads * n_splits * (head_dim + 2) floats).
 extern "C" int cpi_attention_prefill_kv8(const void* q, void* out, const void* k_pages, const void* v_pages, long n_pages,
                                          const int* earlier_table, const int* exact_table, int width, const int* token_seq,
                                          const int* token_pos, const int* tile_tok0, const int* tile_rows, int n_tiles, int n_tokens,
                                          int n_heads, int n_kv_heads, int head_dim, int window_kind, int window_size, int keep_first,
-                                         float scale, float softcap, const float* sink, int* error_flag, cudaStream_t stream) {
+                                         float scale, float softcap, const float* sink, int n_splits, float* scratch, int* error_flag,
+                                         cudaStream_t stream) {
   if (n_tiles == 0) return 0;
+  const long rows = (long)n_tokens * n_heads;
+  CPI_REQUIRE(n_splits >= 1 && n_splits <= 32 && (n_splits == 1 || scratch), "attention_prefill_kv8: %d shares (up to 32, with scratch)", n_splits);
   CPI_REQUIRE(cpi_attention_prefill_supported(n_heads, n_kv_heads, head_dim, pre::PAGE),
               "attention_prefill_kv8: unsupported shape (heads %d/%d, head size %d)", n_heads, n_kv_heads, head_dim);
   CPI_REQUIRE(window_kind == 0 || window_size > 0, "attention_prefill_kv8: window kind %d needs a size > 0", window_kind);
@@ -523,8 +594,9 @@ extern "C" int cpi_attention_prefill_kv8(const void* q, void* out, const void* k
   pre::Params p{(__nv_bfloat16*)out, earlier_table, width, token_pos, token_seq, nullptr, tile_tok0, tile_rows,
                 n_heads, n_kv_heads, window_kind, window_size, scale * 1.4426950408889634f, error_flag, sink,
                 keep_first > 0 ? keep_first : 0, softcap > 0.f ? scale / softcap : 0.f,
-                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, exact_table, (int)n_pages};
-  dim3 grid(n_heads, n_tiles);
+                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, exact_table, (int)n_pages, n_splits, scratch,
+                scratch ? reinterpret_cast<float2*>(scratch + rows * n_splits * head_dim) : nullptr};
+  dim3 grid(n_heads, n_tiles, n_splits);
   const int smem = head_dim / 64 * 128 * 128 * (2 + pre::kRingSlots);
   auto launch = [&](auto dim, auto capped) {
     auto* kernel = pre::attention_prefill_kernel<dim.value, capped.value, true>;
@@ -540,5 +612,9 @@ extern "C" int cpi_attention_prefill_kv8(const void* q, void* out, const void* k
     if (p.cap_out > 0.f) launch(dim, std::true_type{}); else launch(dim, std::false_type{});
   };
   if (head_dim == 128) launch_dim(std::integral_constant<int, 128>{}); else launch_dim(std::integral_constant<int, 64>{});
-  return check_launch("attention_prefill_kv8");
+  if (check_launch("attention_prefill_kv8")) return 2;
+  if (n_splits == 1) return 0;
+  auto* combine = head_dim == 128 ? pre::attention_prefill_combine<128> : pre::attention_prefill_combine<64>;
+  cpi::launch_pdl(combine, dim3((unsigned)((rows + 7) / 8)), 256, 0, stream, p.part_o, p.part_ml, p.out, rows, n_splits, sink, n_heads);
+  return check_launch("attention_prefill_combine");
 }

@@ -1085,49 +1085,75 @@ def attention_decode(q, out, k_cache, v_cache, page_table, page_size, token_seq,
 
 
 # ---- the cache in 8 bits (see cpi_b200/cache/kv8.py for what it holds) ----------------------------------------------------
+# A call of these and of `log_probs` may take a few microseconds on the device, less than its own way there: arguments are declared
+# once (`_declared`), so that plain integers and floats go through without an object each, and checks read each tensor once.
+_INT, _LONG, _FLOAT, _PTR = c_int, c_long, c_float, c_void_p
+_KV8_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+
+
+@functools.lru_cache(maxsize=None)
+def _declared(name: str, types: str):
+    """The library's function `name` with its arguments declared: p a pointer (int or None), i int, l long, f float."""
+    fn = getattr(load(), name)
+    fn.argtypes = [{"p": _PTR, "i": _INT, "l": _LONG, "f": _FLOAT}[t] for t in types]
+    return fn
+
+
+def _run(fn, *args):
+    global launch_count
+    if fn(*args):
+        raise KernelError(load().cpi_last_error().decode())
+    launch_count += 1
+
+
+def _here(what, *ts):
+    """Kernels are launched on the current device's stream: all of a call's tensors have to be there.  Returns the device's number."""
+    here = torch._C._cuda_getDevice() if any(t.is_cuda for t in ts) else -1
+    for t in ts:
+        if t.get_device() != here or here < 0:
+            _need_cuda(t)
+            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{here}")
+    return here
+
+
 def _kv8(cache, what, n_heads=None):
-    """(format, kv heads, head size) of a Kv8Cache after its checks; `n_heads`: the query heads that read it."""
-    codes = {torch.int8: 0, torch.float8_e4m3fn: 1}
-    k, v = cache.k, cache.v
-    if k.dtype not in codes or v.dtype != k.dtype or k.dim() != 4 or k.shape != v.shape:
+    """(format, kv heads, head size, the tensors' addresses) of a Kv8Cache after its checks; `n_heads`: the query heads that read it."""
+    k, v, k_scale, v_scale, k_tail, v_tail = cache
+    shape, fmt = k.shape, _KV8_CODES.get(k.dtype)
+    if fmt is None or v.dtype is not k.dtype or len(shape) != 4 or v.shape != shape:
         raise KernelError(f"{what}: codes are int8 or float8_e4m3fn [pages, kv heads, 64, head size], keys and values alike, not "
-                          f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
-    pages, nkv, block, d = k.shape
+                          f"{tuple(shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    pages, nkv, block, d = shape
     if block != 64 or d not in (64, 128) or pages < 1 or nkv < 1:
-        raise KernelError(f"{what}: pages of 64 positions and heads of 64 or 128 elements, not {tuple(k.shape)}")
-    for t in (cache.k_scale, cache.v_scale):
-        if t.dtype != torch.float32 or t.shape != (pages, nkv):
-            raise KernelError(f"{what}: scales are float32 [{pages}, {nkv}], not {tuple(t.shape)} {t.dtype}")
-    for t in (cache.k_tail, cache.v_tail):
-        if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[1:] != (nkv, 64, d) or t.shape != cache.k_tail.shape:
-            raise KernelError(f"{what}: tails are bfloat16 [slots, {nkv}, 64, {d}], not {tuple(t.shape)} {t.dtype}")
-    for t in cache:
-        if not t.is_contiguous() or t.data_ptr() % 16:
-            raise KernelError(f"{what}: the cache's tensors are contiguous and start on 16 bytes")
+        raise KernelError(f"{what}: pages of 64 positions and heads of 64 or 128 elements, not {tuple(shape)}")
+    f32, bf16 = torch.float32, torch.bfloat16
+    if k_scale.dtype is not f32 or v_scale.dtype is not f32 or k_scale.shape != (pages, nkv) or v_scale.shape != (pages, nkv):
+        raise KernelError(f"{what}: scales are float32 [{pages}, {nkv}], not {tuple(k_scale.shape)} {k_scale.dtype} and {tuple(v_scale.shape)} "
+                          f"{v_scale.dtype}")
+    tail = k_tail.shape
+    if k_tail.dtype is not bf16 or v_tail.dtype is not bf16 or v_tail.shape != tail or len(tail) != 4 or tail[1:] != (nkv, 64, d):
+        raise KernelError(f"{what}: tails are bfloat16 [slots, {nkv}, 64, {d}], not {tuple(tail)} {k_tail.dtype} and {tuple(v_tail.shape)} "
+                          f"{v_tail.dtype}")
+    at = [t.data_ptr() for t in cache]
+    if (at[0] | at[1] | at[2] | at[3] | at[4] | at[5]) % 16 or not (
+            k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous() and k_tail.is_contiguous()
+            and v_tail.is_contiguous()):
+        raise KernelError(f"{what}: the cache's tensors are contiguous and start on 16 bytes")
     if n_heads is not None and (n_heads < 1 or n_heads % nkv or n_heads // nkv > 16):
         raise KernelError(f"{what}: {n_heads} query heads over {nkv} key/value heads (groups of 1 to 16)")
-    return codes[k.dtype], nkv, d
+    return fmt, nkv, d, at
 
 
-def _on_current_device(what, *ts):
-    """Kernels are launched on the current device's stream: all of a call's tensors have to be there."""
-    _need_cuda(*ts)
-    here = torch._C._cuda_getDevice()
+def _i32(what, n, *ts):
     for t in ts:
-        if t is not None and t.device.index != here:
-            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{here}")
+        if t.dtype is not torch.int32 or not t.is_contiguous() or (n is not None and t.numel() != n):
+            raise KernelError(f"{what}: indices are contiguous int32" + ("" if n is None else f" [{n}]") + f", not {t.dtype} {tuple(t.shape)}")
 
 
-def _i32(what, n, **ts):
-    for name, t in ts.items():
-        if t.dtype != torch.int32 or not t.is_contiguous() or (n is not None and t.numel() != n):
-            raise KernelError(f"{what}: {name} is contiguous int32" + ("" if n is None else f" [{n}]") + f", not {t.dtype} {tuple(t.shape)}")
-
-
-def _bf16_rows(what, shape, **ts):
-    for name, t in ts.items():
-        if t.dtype != torch.bfloat16 or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.data_ptr() % 16:
-            raise KernelError(f"{what}: {name} is contiguous bfloat16 {tuple(shape)} from 16 bytes on, not {t.dtype} {tuple(t.shape)}")
+def _bf16_rows(what, shape, *ts):
+    for t in ts:
+        if t.dtype is not torch.bfloat16 or t.shape != shape or not t.is_contiguous() or t.data_ptr() % 16:
+            raise KernelError(f"{what}: expected contiguous bfloat16 {tuple(shape)} from 16 bytes on, not {t.dtype} {tuple(t.shape)}")
 
 
 def _attention_options(what, n_heads, scale, window_kind, window_size, keep_first, sink, softcap):
@@ -1135,8 +1161,21 @@ def _attention_options(what, n_heads, scale, window_kind, window_size, keep_firs
         raise KernelError(f"{what}: window kind {window_kind} of size {window_size}")
     if keep_first < 0 or not scale > 0 or softcap is not None and softcap < 0:
         raise KernelError(f"{what}: keep_first {keep_first}, scale {scale}, softcap {softcap}")
-    if sink is not None and (sink.dtype != torch.float32 or not sink.is_contiguous() or sink.numel() != n_heads):
+    if sink is not None and (sink.dtype is not torch.float32 or not sink.is_contiguous() or sink.numel() != n_heads):
         raise KernelError(f"{what}: a sink is float32 [{n_heads}]")
+
+
+_flag_ptrs = {}       # device number -> address of its error word (the tensor lives in _errors for good)
+
+
+def _flag(here: int) -> int:
+    if here not in _flag_ptrs:
+        _flag_ptrs[here] = tc_error_flag(torch.device("cuda", here)).data_ptr()
+    return _flag_ptrs[here]
+
+
+def _raw_stream(here: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(here)
 
 
 def attention_decode_kv8_supported(n_heads, n_kv_heads, head_dim, page_size) -> bool:
@@ -1149,36 +1188,37 @@ def attention_decode_kv8(q, out, cache, page_table, token_seq, token_pos, seq_sl
     Kv8Cache whose tails hold the new tokens' keys and values already.  A token at position p = 64 b + 63 completes its block:
     the tail's codes and scales are written to page page_table[slot, b].  `max_context`: no sequence is longer (it sizes the
     division of the keys over blocks of threads; any number is right, a good one is fast).  Windows, kept first positions,
-    sink and soft cap as in `attention_decode`.  A token at a negative position is a padded row: its output is zero."""
+    sink and soft cap as in `attention_decode`.  A token at a negative position is a padded row: its output is zero.  Tokens
+    of a call belong to different slots."""
     what = "attention_decode_kv8"
-    fmt, nkv, d = _kv8(cache, what, n_heads)
-    T = q.shape[0]
-    _on_current_device(what, q, out, *cache, page_table, token_seq, token_pos, seq_slot, sink)
-    _bf16_rows(what, (T, n_heads * d), q=q, out=out)
-    _i32(what, T, token_seq=token_seq, token_pos=token_pos)
-    _i32(what, None, seq_slot=seq_slot, page_table=page_table)
-    if page_table.dim() != 2 or T > 65535:
-        raise KernelError(f"{what}: a page table [slots, blocks] and up to 65535 tokens, not {tuple(page_table.shape)} and {T}")
+    fmt, nkv, d, at = _kv8(cache, what, n_heads)
+    T, k_tail = q.shape[0], cache.k_tail
+    here = _here(what, q, out, *cache, page_table, token_seq, token_pos, seq_slot)
+    if sink is not None:
+        _here(what, sink)
+    _bf16_rows(what, (T, n_heads * d), q, out)
+    _i32(what, T, token_seq, token_pos)
+    _i32(what, None, seq_slot, page_table)
+    table = page_table.shape
+    if len(table) != 2 or T > 65535 or table[0] < k_tail.shape[0]:
+        raise KernelError(f"{what}: a page table [slots, blocks] for {k_tail.shape[0]} slots and up to 65535 tokens, not {tuple(table)} and {T}")
     _attention_options(what, n_heads, scale, window_kind, window_size, keep_first, sink, softcap)
-    if page_table.shape[0] < cache.k_tail.shape[0]:
-        raise KernelError(f"{what}: a page table of {page_table.shape[0]} slots, tails of {cache.k_tail.shape[0]}")
     if T == 0:
         return
-    longest = min(int(max_context), page_table.shape[1] * 64)
+    longest = min(int(max_context), table[1] * 64)
     if window_kind != WINDOW_FULL:
         longest = min(longest, window_size + 64 + -(-keep_first // 64) * 64)
-    splits = _kv8_splits(T * nkv, -(-max(longest, 1) // 64), n_heads // nkv)
-    scratch = None
-    if splits > 1:
-        scratch = torch.empty(T * n_heads * splits * (d + 2), dtype=torch.float32, device=q.device)
-    _call("cpi_attention_decode_kv8", _p(q), _p(out), _p(cache.k), _p(cache.v), _p(cache.k_scale), _p(cache.v_scale), c_int(cache.k.shape[0]),
-          _p(cache.k_tail), _p(cache.v_tail), c_int(cache.k_tail.shape[0]), _p(page_table), c_int(page_table.shape[1]), _p(token_seq),
-          _p(token_pos), _p(seq_slot), c_int(seq_slot.numel()), c_int(T), c_int(n_heads), c_int(nkv), c_int(d), c_int(fmt),
-          c_int(window_kind), c_int(int(window_size)), c_int(int(keep_first)), c_float(float(scale)), c_float(float(softcap or 0.0)),
-          _p(sink), c_int(splits), _p(scratch), _p(tc_error_flag(q.device)), _stream())
+    splits = _kv8_splits(here, T * nkv, -(-max(longest, 1) // 64), n_heads // nkv)
+    scratch = None if splits == 1 else torch.empty(T * n_heads * splits * (d + 2), dtype=torch.float32, device=q.device)
+    _run(_declared("cpi_attention_decode_kv8", "ppppppippipipppiiiiiiiiiffpippp"),
+         q.data_ptr(), out.data_ptr(), at[0], at[1], at[2], at[3], cache.k.shape[0], at[4], at[5], k_tail.shape[0], page_table.data_ptr(), table[1],
+         token_seq.data_ptr(), token_pos.data_ptr(), seq_slot.data_ptr(), seq_slot.numel(), T, n_heads, nkv, d, fmt, window_kind, int(window_size),
+         int(keep_first), scale, softcap or 0.0, None if sink is None else sink.data_ptr(), splits, None if scratch is None else scratch.data_ptr(),
+         _flag(here), _raw_stream(here))
 
 
-def _kv8_splits(base: int, pages: int, group: int) -> int:
+@functools.lru_cache(maxsize=4096)
+def _kv8_splits(device: int, base: int, pages: int, group: int) -> int:
     """Blocks of threads that share a sequence's keys, for `base` (token, kv head) pairs of up to `pages` pages each."""
     slots = load().cpi_attention_decode_kv8_blocks_per_sm(c_int(group)) * sm_count()
     want = slots // base if base <= slots else -(-4 * slots // base)
@@ -1191,15 +1231,16 @@ def kv8_stage(cache, page_table, plan, k_pages, v_pages):
     behind them, writes the blocks that are complete now to the cache and each sequence's open block to its tail, and puts
     the numbers that earlier blocks stand for into the earlier pages."""
     what = "kv8_stage"
-    fmt, nkv, d = _kv8(cache, what)
-    _on_current_device(what, *cache, page_table, plan.jobs, k_pages, v_pages)
-    _bf16_rows(what, (plan.n_pages, nkv, 64, d), k_pages=k_pages, v_pages=v_pages)
-    _i32(what, None, page_table=page_table)
-    if page_table.dim() != 2 or page_table.shape[0] < cache.k_tail.shape[0] or page_table.shape[1] < plan.width:
-        raise KernelError(f"{what}: a page table {tuple(page_table.shape)} for {cache.k_tail.shape[0]} slots and blocks up to {plan.width}")
-    _call("cpi_kv8_stage", _p(plan.jobs), c_int(plan.n_jobs), _p(page_table), c_int(page_table.shape[1]), c_int(cache.k_tail.shape[0]),
-          _p(cache.k), _p(cache.v), _p(cache.k_scale), _p(cache.v_scale), c_int(cache.k.shape[0]), _p(cache.k_tail), _p(cache.v_tail),
-          _p(k_pages), _p(v_pages), c_int(plan.n_pages), c_int(nkv), c_int(d), c_int(fmt), _p(tc_error_flag(k_pages.device)), _stream())
+    fmt, nkv, d, at = _kv8(cache, what)
+    slots, table = cache.k_tail.shape[0], page_table.shape
+    here = _here(what, *cache, page_table, plan.jobs, k_pages, v_pages)
+    _bf16_rows(what, (plan.n_pages, nkv, 64, d), k_pages, v_pages)
+    _i32(what, None, page_table)
+    if len(table) != 2 or table[0] < slots or table[1] < plan.width:
+        raise KernelError(f"{what}: a page table {tuple(table)} for {slots} slots and blocks up to {plan.width}")
+    _run(_declared("cpi_kv8_stage", "pipiippppippppiiiipp"), plan.jobs.data_ptr(), plan.n_jobs, page_table.data_ptr(), table[1], slots, at[0], at[1],
+         at[2], at[3], cache.k.shape[0], at[4], at[5], k_pages.data_ptr(), v_pages.data_ptr(), plan.n_pages, nkv, d, fmt, _flag(here),
+         _raw_stream(here))
 
 
 def attention_prefill_kv8(q, out, k_pages, v_pages, plan, token_seq, token_pos, tile_tok0, tile_rows, *, n_heads, scale,
@@ -1208,24 +1249,38 @@ def attention_prefill_kv8(q, out, k_pages, v_pages, plan, token_seq, token_pos, 
     positions in the exact pages and earlier ones in the earlier pages.  q, out bfloat16 [T, n_heads * head_dim]; query
     tiles as in `attention_prefill`; the window is the plan's."""
     what = "attention_prefill_kv8"
-    if k_pages.dim() != 4 or k_pages.shape[2] != 64 or k_pages.shape[3] not in (64, 128):
-        raise KernelError(f"{what}: pages [pages, kv heads, 64, 64 or 128], not {tuple(k_pages.shape)}")
-    nkv, d = k_pages.shape[1], k_pages.shape[3]
-    if n_heads < 1 or n_heads % nkv:
+    shape = k_pages.shape
+    if len(shape) != 4 or shape[2] != 64 or shape[3] not in (64, 128):
+        raise KernelError(f"{what}: pages [pages, kv heads, 64, 64 or 128], not {tuple(shape)}")
+    nkv, d = shape[1], shape[3]
+    if n_heads < 1 or nkv < 1 or n_heads % nkv:
         raise KernelError(f"{what}: {n_heads} query heads over {nkv} key/value heads")
-    _on_current_device(what, q, out, k_pages, v_pages, plan.jobs, token_seq, token_pos, tile_tok0, tile_rows, sink)
-    _bf16_rows(what, (plan.n_tokens, n_heads * d), q=q, out=out)
-    _bf16_rows(what, (plan.n_pages, nkv, 64, d), k_pages=k_pages, v_pages=v_pages)
-    _i32(what, plan.n_tokens, token_seq=token_seq, token_pos=token_pos)
-    _i32(what, tile_tok0.numel(), tile_tok0=tile_tok0, tile_rows=tile_rows)
+    here = _here(what, q, out, k_pages, v_pages, plan.jobs, token_seq, token_pos, tile_tok0, tile_rows)
+    if sink is not None:
+        _here(what, sink)
+    _bf16_rows(what, (plan.n_tokens, n_heads * d), q, out)
+    _bf16_rows(what, (plan.n_pages, nkv, 64, d), k_pages, v_pages)
+    _i32(what, plan.n_tokens, token_seq, token_pos)
+    tiles = tile_tok0.numel()
+    _i32(what, tiles, tile_tok0, tile_rows)
     _attention_options(what, n_heads, scale, window_kind, window_size, keep_first, sink, softcap)
-    names = {v: k for k, v in WINDOW_KINDS.items()}
-    if (names[window_kind], window_size if window_kind != WINDOW_FULL else 0, keep_first if window_kind == WINDOW_SLIDING else 0) != plan.window:
-        raise KernelError(f"{what}: window {names[window_kind]} of {window_size}, {keep_first} kept: the plan was made for {plan.window}")
-    _call("cpi_attention_prefill_kv8", _p(q), _p(out), _p(k_pages), _p(v_pages), c_long(plan.n_pages), _p(plan.earlier_table),
-          _p(plan.exact_table), c_int(plan.width), _p(token_seq), _p(token_pos), _p(tile_tok0), _p(tile_rows), c_int(tile_tok0.numel()),
-          c_int(plan.n_tokens), c_int(n_heads), c_int(nkv), c_int(d), c_int(window_kind), c_int(int(window_size)), c_int(int(keep_first)),
-          c_float(float(scale)), c_float(float(softcap or 0.0)), _p(sink), _p(tc_error_flag(q.device)), _stream())
+    window = (window_kind, window_size if window_kind else 0, keep_first if window_kind == WINDOW_SLIDING else 0)
+    if window != (WINDOW_KINDS[plan.window[0]], *plan.window[1:]):
+        raise KernelError(f"{what}: window kind {window_kind} of {window_size}, {keep_first} kept: the plan was made for {plan.window}")
+    splits = _kv8_prefill_splits(here, tiles * n_heads, plan.most_tiles)
+    scratch = None if splits == 1 else torch.empty(plan.n_tokens * n_heads * splits * (d + 2), dtype=torch.float32, device=q.device)
+    _run(_declared("cpi_attention_prefill_kv8", "pppplppippppiiiiiiiiffpippp"), q.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+         plan.n_pages, plan.earlier_table.data_ptr(), plan.exact_table.data_ptr(), plan.width, token_seq.data_ptr(), token_pos.data_ptr(),
+         tile_tok0.data_ptr(), tile_rows.data_ptr(), tiles, plan.n_tokens, n_heads, nkv, d, window_kind, int(window_size), int(keep_first), scale,
+         softcap or 0.0, None if sink is None else sink.data_ptr(), splits, None if scratch is None else scratch.data_ptr(), _flag(here),
+         _raw_stream(here))
+
+
+@functools.lru_cache(maxsize=4096)
+def _kv8_prefill_splits(device: int, blocks: int, tiles: int) -> int:
+    """Blocks of threads that share the keys of a query tile: `blocks` of them would run (one to an SM), over up to `tiles` key
+    tiles of 128 positions each.  A share holds four tiles or more: joining the shares costs about two."""
+    return max(1, min(sm_count() // max(blocks, 1), tiles // 4, 32))
 
 
 def latent_attention_supported(row: int, rank: int) -> bool:
@@ -1462,6 +1517,11 @@ def ban_tokens(logits, ids, id_offsets):
           _stream())
 
 
+@functools.lru_cache(maxsize=None)
+def _log_probs_most() -> int:
+    return int(load().cpi_log_probs_max_top())
+
+
 class LogProbs(NamedTuple):
     logprob: torch.Tensor                # float32, shaped as the targets: log p of each
     entropy: torch.Tensor                # float32 [rows], in nats
@@ -1482,16 +1542,18 @@ def log_probs(logits, targets, *, top=0):
     if targets.dtype not in (torch.int32, torch.int64) or targets.dim() not in (1, 2) or targets.shape[0] != R or not targets.is_contiguous():
         raise KernelError(f"{what}: targets are contiguous int32 or int64 [{R}] or [{R}, n], not {targets.dtype} {tuple(targets.shape)}")
     top = int(top)
-    most = int(load().cpi_log_probs_max_top())
+    most = _log_probs_most()
     if not 0 <= top <= min(most, V):
         raise KernelError(f"{what}: top {top} of a vocabulary of {V} (at most {most})")
-    _on_current_device(what, logits, targets)
-    dev = logits.device
-    out = LogProbs(torch.empty(targets.shape, dtype=torch.float32, device=dev), torch.empty(R, dtype=torch.float32, device=dev),
-                   torch.empty((R, top), dtype=torch.float32, device=dev) if top else None,
-                   torch.empty((R, top), dtype=torch.int32, device=dev) if top else None)
+    here = _here(what, logits, targets)
+    n = targets.numel()
+    # (one allocation for all of them: three more cost as much as the launch)
+    buf = torch.empty(n + R * (1 + 2 * top), dtype=torch.float32, device=logits.device)
+    out = LogProbs(buf.as_strided(targets.shape, targets.stride(), 0), buf.as_strided((R,), (1,), n),
+                   buf.as_strided((R, top), (top, 1), n + R) if top else None,
+                   buf.view(torch.int32).as_strided((R, top), (top, 1), n + R * (1 + top)) if top else None)
     if R:
-        _call("cpi_log_probs", _p(logits), c_int(dtype_code(logits.dtype)), c_long(logits.stride(0)), c_int(R), c_int(V), _p(targets),
-              c_int(1 if targets.dim() == 1 else targets.shape[1]), c_int(int(targets.dtype == torch.int64)), _p(out.logprob), _p(out.entropy),
-              _p(out.top_logprobs), _p(out.top_ids), c_int(top), _stream())
+        _run(_declared("cpi_log_probs", "piliipiippppip"), logits.data_ptr(), dtype_code(logits.dtype), logits.stride(0), R, V, targets.data_ptr(),
+             1 if targets.dim() == 1 else targets.shape[1], int(targets.dtype is torch.int64), out.logprob.data_ptr(), out.entropy.data_ptr(),
+             out.top_logprobs.data_ptr() if top else None, out.top_ids.data_ptr() if top else None, top, _raw_stream(here))
     return out

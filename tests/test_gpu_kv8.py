@@ -297,6 +297,21 @@ def test_later_pieces(how, pasts, news):
         rig.check_held(i)
 
 
+@pytest.mark.parametrize("nh,nkv,d,past,news", [(1, 1, 64, 3000, [2]), (2, 1, 128, 2111, [300]), (4, 4, 64, 5000, [130, 64]), (2, 2, 128, 1300, [1, 513])])
+@pytest.mark.parametrize("how", [dict(), dict(window="sliding", size=1500, keep=70), dict(window="chunk", size=1000)])
+def test_few_query_tiles_over_long_contexts(nh, nkv, d, past, news, how):
+    """Few blocks of threads over many keys: a query tile's keys are shared out, with sinks and without."""
+    rig = Rig([past + n for n in news], fmt="e4m3", nh=nh, nkv=nkv, d=d, seed=past)
+    for i in range(len(news)):
+        rig.load(i, past)
+    sink = torch.linspace(-2, 6, nh, device=DEV) if nh > 2 else None
+    q, out, starts = rig.prompt(news, sink=sink, **how)
+    for i, (s, n) in enumerate(zip(starts, news)):
+        some = sorted({0, 1, n // 2, n - 1, 63, 64, 127, 128, 255, 256} & set(range(n)))
+        rig.check(i, q[i][some], out[i][some], [s + x for x in some], sink=sink, **how)
+        rig.check_held(i)
+
+
 @pytest.mark.parametrize("softcap", [0.0, 8.0])
 def test_prompt_sink_and_cap(softcap):
     rig = Rig([300], nh=8, nkv=2, d=64, seed=12)

@@ -122,3 +122,17 @@ def test_calls_refuse_the_host():
 def test_log_probs_refusals(logits, targets, top):
     with pytest.raises(K.KernelError):
         K.log_probs(logits, targets, top=top)
+
+
+def test_arguments_are_declared_as_the_library_has_them():
+    """The kinds that a binding declares are those of the C function, one for one."""
+    import os
+    import re
+    folder = os.path.dirname(K.__file__)
+    sources = "".join(open(os.path.join(folder, f)).read() for f in sorted(os.listdir(folder)) if f.endswith(".cu"))
+    declared = re.findall(r'_declared\("(\w+)", "(\w+)"\)', open(K.__file__).read())
+    assert len(declared) >= 4
+    for name, types in declared:
+        args = re.search(r'extern "C" int ' + name + r"\(([^)]*)\)", sources).group(1).split(",")
+        kinds = ["p" if "*" in a or "cudaStream_t" in a else "f" if "float " in a else "l" if "long " in a else "i" for a in args]
+        assert "".join(kinds) == types, name
