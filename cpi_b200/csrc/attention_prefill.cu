@@ -64,6 +64,10 @@ struct Params {
 };
 
 
+// BLOCKED raises a row's reference only by 2^40: P is bfloat16 and the sums are float32, which have the same range of powers, so
+// nothing is lost by numbers up to 2^40 (sums up to 2^57, outputs finite for values up to 2^70), and a pass is hardly ever
+// repeated (keys and queries with a few large features, 3,001 tokens of 40 heads: 190 us with 2^8, 171 with 2^40).
+constexpr float kWideSlack = 40.0f;
 constexpr int kRingSlots = 5;           // key and value tiles in shared memory at a time
 
 template <int D, bool CAPPED, bool BLOCKED = false>
@@ -332,6 +336,94 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
         }
         return in;
       };
+      if constexpr (BLOCKED) {
+        // Small code: a block of threads meets most of it cold, and with masks on several tiles, exact and earlier ones, the
+        // pass below, four times over, is more than an instruction cache holds.  Tiles without a mask take one pass of their
+        // own against the reference they have; all others two small loops, the maximum and then the exponentials, whose
+        // P goes over columns of S that have been read.  Columns that no row of the warp sees are passed over.
+        bool stored = false;
+        auto raised = [&](float mx) {                      // the reference after a row maximum mx; O follows
+          const bool grow = mx > m_ref + (m_ref < -1e29f ? 0.f : kWideSlack);
+          if (j == 0) { m_ref = fmaxf(mx, m_ref); return; }
+          if (!__any_sync(0xffffffffu, grow)) return;
+          const float m_new = grow ? mx : m_ref, f = exp2f(m_ref - m_new);
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {                // (every P V issued so far has landed, see below)
+            float v[32];
+            tmem_ld32(o_row + c, v);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] *= f;
+            tmem_st32(o_row + c, v);
+          }
+          l_run *= f;
+          m_ref = m_new;
+        };
+        if (!CAPPED && no_mask && j > 0) {
+          uint32_t w[BKV / 32][16], raw[2][32];
+          const float nref = -m_ref;
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, ls4[4] = {0.f, 0.f, 0.f, 0.f};
+          tmem_ld32_issue(s_row, raw[0]);
+          tmem_ld32_issue(s_row + 32, raw[1]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int cc = 0; cc < BKV / 32; ++cc) {
+            float v[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float sv = __uint_as_float(raw[cc & 1][e]);
+              mx4[e & 3] = fmaxf(mx4[e & 3], sv);
+              v[e] = exp2_fast(fmaf(sv, sc, nref));
+            }
+            if (cc + 2 < BKV / 32) tmem_ld32_issue(s_row + (cc + 2) * 32, raw[cc & 1]);     // this buffer is consumed
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ls4[e & 3] += v[e];
+#pragma unroll
+            for (int g = 0; g < 16; ++g) w[cc][g] = pack_bf16(v[2 * g], v[2 * g + 1]);
+            if (cc == 1) tmem_wait_ld();
+          }
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+          stored = !__any_sync(0xffffffffu, mx > m_ref + (m_ref < -1e29f ? 0.f : kWideSlack));
+          if (stored) {
+#pragma unroll
+            for (int cc = 0; cc < BKV / 32; ++cc) tmem_st16_nowait(s_row + cc * 16, w[cc]);
+            l_run += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
+          }
+        }
+        if (!stored) {
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < BKV; c += 32) {
+            const uint32_t in = no_mask ? 0xffffffffu : sees(key0 + c);
+            if (!__any_sync(0xffffffffu, in != 0)) continue;
+            float v[32], mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_ld32(s_row + c, v);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], (in >> e) & 1u ? v[e] : -INFINITY);
+            mx = fmaxf(mx, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
+          }
+          raised(CAPPED && mx > -INFINITY ? tanh_fast(mx * cap_in) * sc : mx * sc);
+          const float nref = -m_ref;
+#pragma unroll 1
+          for (int c = 0; c < BKV; c += 32) {
+            const uint32_t in = no_mask ? 0xffffffffu : sees(key0 + c);
+            uint32_t w[16] = {};
+            if (__any_sync(0xffffffffu, in != 0)) {
+              float v[32], ls4[4] = {0.f, 0.f, 0.f, 0.f};
+              tmem_ld32(s_row + c, v);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                if (CAPPED) v[e] = tanh_fast(v[e] * cap_in);
+                v[e] = (in >> e) & 1u ? exp2_fast(fmaf(v[e], sc, nref)) : 0.f;
+                ls4[e & 3] += v[e];
+              }
+#pragma unroll
+              for (int g = 0; g < 16; ++g) w[g] = pack_bf16(v[2 * g], v[2 * g + 1]);
+              l_run += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
+            }
+            tmem_st16_nowait(s_row + (c >> 1), w);
+          }
+        }
+      } else {
       // One pass over the row's 128 columns of S, 32 at a time with the next chunk's load in flight: the
       // maximum, P = 2^(s c - ref) as packed bf16, and the sum.  P is kept in registers until the pass is
       // known to stand, because it goes over the S it came from.
@@ -344,9 +436,8 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
 #pragma unroll 1
         for (int c = 0; c < BKV; c += 32) {
           float v[32], mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          const uint32_t in = sees(key0 + c);
-          if (BLOCKED && !__any_sync(0xffffffffu, in != 0)) continue;       // (no row of the warp sees a column of it)
           tmem_ld32(s_row + c, v);
+          const uint32_t in = sees(key0 + c);
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             if (CAPPED) v[e] = tanh_fast(v[e] * cap_in);
@@ -376,10 +467,6 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
             }
           } else {
             const uint32_t in = sees(key0 + cc * 32);
-            if (BLOCKED && !__any_sync(0xffffffffu, in != 0)) {             // (no row of the warp sees a column of it)
-#pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = 0.f;
-            } else
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               float sv = __uint_as_float(raw[cc & 1][e]);
@@ -423,6 +510,7 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
 #pragma unroll
       for (int cc = 0; cc < BKV / 32; ++cc) tmem_st16_nowait(s_row + cc * 16, w[cc]);
       l_run += ls;
+      }
       tmem_wait_st();
       fence_before_sync();
       __syncwarp();
