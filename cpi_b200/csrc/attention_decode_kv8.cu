@@ -1,25 +1,31 @@
 // Decode attention over the cache in 8 bits (kv8.cuh): one new token per sequence, its own block of 64 positions in bfloat16 (the
 // sequence's tail), the complete blocks before it as codes with a scale per block and head.
 //
-// A block of threads serves one (split, key/value head, token).  A fifth warp streams (page, head) tiles of codes (64 x D bytes of
-// keys, as many of values; TMA boxes of 128 bytes with the 128-byte swizzle) into a ring of shared-memory stages; four warps take
-// 16 positions of each tile and run an online softmax of their own:
-//     S^T = K Q^T     m16n8k16 with the positions as M and the group's heads as N (8, or twice 8): with heads as M half of the
-//                     rows would be empty in the usual groups of 4 to 8, and a lane then holds the maxima of the heads that its
-//                     outputs belong to.  The codes become float16 in registers: an int8 c as 1024 + (c + 128) by putting its byte
-//                     under the exponent of 1024, less 1152; e4m3 by the hardware's conversion; both exact.  Which positions of k
-//                     a lane's bytes fill is free as long as Q's do the same, so four neighbouring bytes of a row need no shuffle.
+// A block of threads serves one (split, key/value head, token).  Its warps take half pages in turn (a tile: 32 positions x D bytes)
+// and stream them through shared-memory slots of their own: keys, values, keys, ... (TMA boxes of 128 bytes with the 128-byte
+// swizzle), the next one asked for as soon as a slot has been read.  A slot's rounds are waited for by one warp, in order: a
+// wait for a parity may be one round behind and no more.  Every warp runs an online softmax of its own:
+//     S^T = K Q^T     m16n8k16 with the positions as M (two tiles of 16) and the group's heads as N (8,
+//                     or twice 8): with heads as M half of the rows would be empty in the usual groups of 4 to 8, and a lane
+//                     then holds the maxima of the heads that its outputs belong to.  The codes become float16 in registers: an int8
+//                     c as 1024 + (c + 128) by putting its byte under the exponent of 1024, less 1152; e4m3 by the hardware's
+//                     conversion; both exact.  Which positions of k a lane's bytes fill is free as long as Q's do the same, so four
+//                     neighbouring bytes of a row need no shuffle.
 //     O^T += V^T P^T  values by transposing loads: a pair of bytes is a pair of features, even features form the upper half of
 //                     M, odd ones the lower.  P^T comes out of S^T's registers by movmatrix.
+// What a warp does for a tile is one long chain of dependent steps, so the count of warps decides: 64 sequences of up to 16,384
+// positions (40/8 heads of 128, e4m3) took 204 us with eight warps an SM at a page each (3,400 cycles a page, the data long there).
 // The queries are float16 too, each head's divided by a power of two (11 bits of significand hold bfloat16's 8 exactly; what is
 // 2^-22 below a head's largest element loses bits).  Scales act on scores in float32; the value scale 2^e enters the exponent: a
 // probability is p = 2^(s + e - m) with m the maximum of s + e, and the sum takes p 2^-e.  So blocks of any scale share one
 // accumulator, at no operation per output.
-// p is rounded to float16 (11 bits) against a reference m that is raised when s + e has outgrown it by 2^8: p <= 2^14, and what
-// is 2^-20 of the largest still has all its bits.  Sums, maxima and outputs are float32.
+// p is rounded to float16 (11 bits) against a reference m that is raised when s + e has outgrown it by 2^8, so the largest p lies
+// between 2^6 and 2^14: what is 2^-20 of the largest still has all its bits, smaller terms are off by 2^-31 of the largest at most.
+// (bfloat16 would keep 8 bits of all of them, but codes cost twice as many operations to become bfloat16.)  Sums, maxima and
+// outputs are float32.
 //
-// The tail: each warp takes 16 positions in bfloat16, straight from memory (one page at most, in the last split).  A token that
-// completes its block (position 63 of 64) has its tail turned into codes by the threads that serve it, for the steps after this one.
+// The tail: four warps take 16 positions each in bfloat16, straight from memory (one page at most, in the last split).  A token
+// that completes its block (position 63 of 64) has its tail turned into codes, for the steps after this one, by the last split.
 // Rows of masked positions are zeros before they are multiplied: what an earlier sequence left cannot reach a result.
 // Waits are bounded as in attention_decode.cu.
 #include "kv8.cuh"
@@ -33,7 +39,6 @@ int get_map_2d_bf16(const void* ptr, uint64_t inner, uint64_t rows, uint64_t row
 namespace dec8 {
 
 using kv8::PAGE;
-constexpr int NT = 160, CONSUMERS = 4;
 constexpr uint32_t kSpinLimit = 1u << 24;
 constexpr float kSlack = 8.f, kLift = 6.f;        // p = 2^(s + e - m + kLift), m raised when s + e exceeds it by kSlack
 constexpr int kTailUnits = 2;                     // a tail's bytes, in pages of codes
@@ -61,9 +66,6 @@ __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
 }
 __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -129,14 +131,6 @@ __device__ __forceinline__ int window_low(int kind, int size, int pos) {
 __device__ __forceinline__ float sink_term(const float* sink, int head, float m) {
   return sink ? exp2f(fminf(sink[head] * 1.4426950408889634f - m + kLift, 120.f)) : 0.f;
 }
-// A barrier of the four consumer warps; whether any of their threads brought `v`.
-__device__ __forceinline__ bool any_consumer(bool v) {
-  int r;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.or.pred.aligned q, 1, 128, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
-               : "=r"(r) : "r"((int)v) : "memory");
-  return r != 0;
-}
-__device__ __forceinline__ void consumers_sync() { asm volatile("barrier.cta.sync.aligned 1, 128;" ::: "memory"); }
 // The four codes of a word as two pairs of float16: bytes (0, 1) and (2, 3), or with SPLIT bytes (0, 2) and (1, 3).
 template <int FMT, bool SPLIT> __device__ __forceinline__ void numbers(uint32_t w, uint32_t& a, uint32_t& b) {
   if (FMT == kv8::kInt8) {
@@ -153,11 +147,16 @@ template <int FMT, bool SPLIT> __device__ __forceinline__ void numbers(uint32_t 
   }
 }
 
-template <int D> struct Shape {
-  static constexpr int TILE = PAGE * D;                     // bytes of a (page, head) tile of codes
-  static constexpr int STAGES = D == 128 ? 4 : 6;
+template <int D, int HT> struct Shape {
+  static constexpr int WARPS = HT == 1 ? 8 : 4;             // (with two tiles of heads a thread needs twice the registers)
+  static constexpr int NT = WARPS * 32;
+  static constexpr int POS = 32;                            // positions of a tile
+  static constexpr int TILE = POS * D;                      // bytes of it
   static constexpr int LINES = TILE / 128;                  // the tile as lines of 128 bytes (one, or half, a position each)
-  static constexpr int RING = STAGES * 2 * TILE;
+  static constexpr int SLOTS = (D == 128 ? 3 : 6) * (HT == 1 ? 1 : 2);       // tiles of keys or values that a warp has on their way or reads
+  static constexpr int RING = WARPS * SLOTS * TILE;
+  static constexpr int MERGE = WARPS * HT * 8 * D * 4;
+  static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + 1024;
 };
 // Byte offset of the 16-byte chunk `c` of position `row` in a tile, as the copy engine's 128-byte swizzle leaves it.
 template <int D> __device__ __forceinline__ uint32_t chunk_at(int row, int c) {
@@ -165,29 +164,56 @@ template <int D> __device__ __forceinline__ uint32_t chunk_at(int row, int c) {
   return (uint32_t)(line * 128 + (((at & 7) ^ (line & 7)) << 4));
 }
 
+// A block of threads turns a token's tails [64, D] into codes and scales, for keys and values.
+template <int D, int FMT, int NT>
+__device__ __forceinline__ void hold_tail(const __nv_bfloat16* k_tail, const __nv_bfloat16* v_tail, uint8_t* k_to, uint8_t* v_to, float* k_scale,
+                                          float* v_scale, uint32_t* top_s) {
+  constexpr int PER = PAGE * D / 8 / NT;
+  const int tid = threadIdx.x;
+  const uint4 *ks = reinterpret_cast<const uint4*>(k_tail), *vs = reinterpret_cast<const uint4*>(v_tail);
+  uint4 k[PER], v[PER];
+  uint32_t tk = 0, tv = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) { k[i] = ks[tid + i * NT]; v[i] = vs[tid + i * NT]; }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) { tk = max(tk, kv8::top_of(k[i])); tv = max(tv, kv8::top_of(v[i])); }
+  tk = __reduce_max_sync(0xffffffffu, tk);
+  tv = __reduce_max_sync(0xffffffffu, tv);
+  if ((tid & 31) == 0) { top_s[tid >> 5] = tk; top_s[8 + (tid >> 5)] = tv; }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) { tk = max(tk, top_s[w]); tv = max(tv, top_s[8 + w]); }
+  const int ek = kv8::scale_exponent<FMT>(__uint_as_float(tk << 16)), ev = kv8::scale_exponent<FMT>(__uint_as_float(tv << 16));
+  const float ik = kv8::power_of_two(-ek), iv = kv8::power_of_two(-ev);
+  uint2 *kd = reinterpret_cast<uint2*>(k_to), *vd = reinterpret_cast<uint2*>(v_to);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) { kd[tid + i * NT] = kv8::codes8<FMT>(k[i], ik); vd[tid + i * NT] = kv8::codes8<FMT>(v[i], iv); }
+  if (tid == 0) { *k_scale = kv8::power_of_two(ek); *v_scale = kv8::power_of_two(ev); }
+}
+
 template <int D, int FMT, int HT>
-__global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) attention_decode_kv8_kernel(const __grid_constant__ CUtensorMap map_k,
-                                                                                   const __grid_constant__ CUtensorMap map_v, Params p) {
-  using S = Shape<D>;
-  constexpr int STAGES = S::STAGES, NC = D / 16;            // NC: 16-byte chunks of a row, steps of k, tiles of M
+__global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                     const __grid_constant__ CUtensorMap map_v, Params p) {
+  using S = Shape<D, HT>;
+  constexpr int WARPS = S::WARPS, NT = S::NT, SLOTS = S::SLOTS, POS = S::POS;
+  constexpr int NC = D / 16, MT = POS / 16;                 // 16-byte chunks of a row (steps of k, tiles of M); tiles of 16 positions
   extern __shared__ uint8_t smem_dyn[];
-  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES];
-  __shared__ float wm[CONSUMERS][HT * 8], wl[CONSUMERS][HT * 8];
-  __shared__ uint32_t top_s[2][CONSUMERS];
+  __shared__ uint64_t full_bar[WARPS * SLOTS];
+  __shared__ float wm[WARPS][HT * 8], wl[WARPS][HT * 8];
+  __shared__ uint32_t top_s[16];
   __shared__ int abort_s;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   const int split = blockIdx.x, kvh = blockIdx.y, t = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, j = lane & 3;
   volatile int* aborted = &abort_s;
   if (tid == 0) {
-    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], CONSUMERS); }
+    for (int s = 0; s < WARPS * SLOTS; ++s) mbar_init(&full_bar[s], 1);
     abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  __syncthreads();
-  pdl_wait();
-  pdl_launch_dependents();                                  // (in this order: it reads cached rows, see common.cuh)
-
+  // Positions, slots and the page table are in place before the kernels in front of this one begin (see common.cuh): they are
+  // read under those kernels' ends, the cache and the queries after them.
   const int G = p.n_heads / p.n_kv_heads;
   int pos = p.token_pos[t];
   const int seq = p.token_seq[t];
@@ -209,50 +235,69 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) attention_decode_kv8_kern
   const int begin = min(n_items, split * per), end = split == p.n_splits - 1 ? n_items : min(n_items, begin + per);
   const bool has_tail = pos >= 0 && split == p.n_splits - 1;
   const int total_pages = p.n_pages;
+  const size_t tail = ((size_t)max(slot, 0) * p.n_kv_heads + kvh) * (PAGE * D);
 
-  if (warp == CONSUMERS) {
-    // ---- the producer: page numbers 32 at a time, then a tile of keys and one of values per item ----
-    int pages = 0;
-    for (int i = begin; i < end; ++i) {
-      const int n = i - begin, st = n % STAGES;
-      if ((n & 31) == 0) {
-        const int at = i + lane;
-        pages = at < end ? table[block_of(at)] : 0;
-        if (pages < 0 || pages >= total_pages) {            // (beyond the map's last row: zeros arrive)
-          pages = total_pages;
-          if (p.error_flag) atomicExch(p.error_flag, 3);
-        }
-      }
-      const int page = __shfl_sync(0xffffffffu, pages, n & 31);
-      int ok = 1;
-      if (lane == 0) {
-        if (n >= STAGES) ok = mbar_wait(&empty_bar[st], ((n / STAGES) - 1) & 1, aborted);
-        if (ok) {
-          const int line = (page * p.n_kv_heads + kvh) * S::LINES;
-          mbar_expect_tx(&full_bar[st], 2 * S::TILE);
-          tma_load_2d(ring + st * 2 * S::TILE, &map_k, &full_bar[st], 0, line);
-          tma_load_2d(ring + st * 2 * S::TILE + S::TILE, &map_v, &full_bar[st], 0, line);
-        }
-      }
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+  // This warp's half pages are number warp, warp + WARPS, ... of the split's; its tiles y = 2 x (keys of its half page x), 2 x + 1 (values)
+  const int halves = 2 * (end - begin);
+  const int mine = max(0, (halves - warp + WARPS - 1) / WARPS);
+  auto half_of = [&](int x) { return warp + x * WARPS; };
+  auto block_at = [&](int x) { return block_of(begin + (half_of(x) >> 1)); };
+  uint8_t* slots = ring + warp * SLOTS * S::TILE;
+  uint64_t* bars = full_bar + warp * SLOTS;
+  int ids = 0;                                              // page numbers of 32 of its half pages, one per lane, for the tiles asked for
+  auto take_ids = [&](int x) {
+    ids = x + lane < mine ? table[block_at(x + lane)] : 0;
+    if (ids < 0 || ids >= total_pages) {                    // (beyond the map's last row: zeros arrive)
+      ids = total_pages;
+      if (p.error_flag) atomicExch(p.error_flag, 3);
     }
-  } else {
-    // ---- the consumers ----
-    const int g = lane >> 2, j = lane & 3;
-    const int key0 = warp * 16;
-    const __nv_bfloat16* q = p.q + ((size_t)t * p.n_heads + (size_t)kvh * G) * D;
+  };
+  auto ask = [&](int y, int at) {                           // tile y into slot `at` (all lanes call it)
+    const int x = y >> 1;
+    if (x >= mine) return;
+    if (y % 64 == 0 && y > 0) take_ids(x);
+    const int page = __shfl_sync(0xffffffffu, ids, x & 31);
+    if (lane == 0) {
+      mbar_expect_tx(&bars[at], S::TILE);
+      tma_load_2d(slots + at * S::TILE, y & 1 ? &map_v : &map_k, &bars[at], 0,
+                  ((page * p.n_kv_heads + kvh) * (PAGE / POS) + (half_of(x) & 1)) * S::LINES);
+    }
+  };
+  take_ids(0);
+  __syncthreads();                                          // the barriers are ready
+  pdl_wait();
+  pdl_launch_dependents();                                  // (in this order: it reads cached rows, see common.cuh)
+#pragma unroll
+  for (int y = 0; y < SLOTS; ++y) ask(y, y);
+  const __nv_bfloat16* q = p.q + ((size_t)t * p.n_heads + (size_t)kvh * G) * D;
+  uint2 raw[HT][NC];
+#pragma unroll
+  for (int h = 0; h < HT; ++h)
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      raw[h][c] = h * 8 + g < G ? *reinterpret_cast<const uint2*>(q + (size_t)(h * 8 + g) * D + c * 16 + 4 * j) : make_uint2(0u, 0u);
+
+  {
+    // the own block: four warps of the last split take 16 of its positions each
+    const int tail0 = own * PAGE + warp * 16;
+    const bool tail_any = has_tail && warp < 4 && tail0 <= pos && (tail0 + 15 >= lo || tail0 < keep);
+    const __nv_bfloat16 *kt_tail = p.k_tail + tail + (warp & 3) * 16 * D, *vt_tail = p.v_tail + tail + (warp & 3) * 16 * D;
+    uint4 tk[NC];                                           // rows g and g + 8, 16 bytes of each two chunks
+    if (tail_any) {
+#pragma unroll
+      for (int c = 0; c < NC; c += 2) {
+        tk[c] = *reinterpret_cast<const uint4*>(kt_tail + g * D + c * 16 + 8 * j);
+        tk[c + 1] = *reinterpret_cast<const uint4*>(kt_tail + (g + 8) * D + c * 16 + 8 * j);
+      }
+    }
     // B operands: column g = head g of the tile (heads beyond the group are zeros), k in the order of a lane's bytes
     uint32_t qf[HT][NC][2];
-    float f[HT][2];                                         // per head of this lane's columns 2j, 2j + 1: 2^(q's power) scale log2(e)
+    float f[HT][2];                                         // per head of this lane's columns 2j, 2j + 1: 2^(q's power)
 #pragma unroll
     for (int h = 0; h < HT; ++h) {
-      uint2 raw[NC];
       uint32_t top = 0;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        raw[c] = h * 8 + g < G ? *reinterpret_cast<const uint2*>(q + (size_t)(h * 8 + g) * D + c * 16 + 4 * j) : make_uint2(0u, 0u);
-        top = max(top, kv8::top_of(make_uint4(raw[c].x, raw[c].y, 0u, 0u)));
-      }
+      for (int c = 0; c < NC; ++c) top = max(top, kv8::top_of(make_uint4(raw[h][c].x, raw[h][c].y, 0u, 0u)));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // the largest element lies in [1, 2) after the division (a subnormal top: as it is, times 2^120)
@@ -260,8 +305,8 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) attention_decode_kv8_kern
       const float inv = kv8::power_of_two(-e);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        qf[h][c][0] = pack_f16(kv8::lo_f32(raw[c].x) * inv, kv8::hi_f32(raw[c].x) * inv);
-        qf[h][c][1] = pack_f16(kv8::lo_f32(raw[c].y) * inv, kv8::hi_f32(raw[c].y) * inv);
+        qf[h][c][0] = pack_f16(kv8::lo_f32(raw[h][c].x) * inv, kv8::hi_f32(raw[h][c].x) * inv);
+        qf[h][c][1] = pack_f16(kv8::lo_f32(raw[h][c].y) * inv, kv8::hi_f32(raw[h][c].y) * inv);
       }
       const float mine = kv8::power_of_two(e);
       f[h][0] = __shfl_sync(0xffffffffu, mine, 8 * j);
@@ -275,35 +320,15 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) attention_decode_kv8_kern
 #pragma unroll
       for (int c = 0; c < NC; ++c) o[h][c][0] = o[h][c][1] = o[h][c][2] = o[h][c][3] = 0.f;
     }
-    // Scores s (S^T fragment of 16 positions from position `first` on) -> p in place, its sums, the reference raised where needed.
-    // `k_unit`: what a unit of s is worth beside q's power; `ev`: log2 of the value scale, `v_inv` = 2^-ev.
-    auto softmax = [&](float (&s)[HT][4], int first, bool ragged, float k_unit, float ev, float v_inv) {
-      bool in0 = true, in1 = true;
-      if (ragged) {
-        const int p0 = first + g, p1 = p0 + 8;
-        in0 = (p0 >= lo || p0 < keep) && p0 <= pos;
-        in1 = (p1 >= lo || p1 < keep) && p1 <= pos;
-      }
+    // The maxima mx of new scores (base 2, the value scale's power in them) over this lane's positions: over all lanes of the
+    // head, and the reference raised where they have outgrown it.
+    auto raise = [&](float (&mx)[HT][2]) {
       bool grow = false;
-      float mx[HT][2];
 #pragma unroll
       for (int h = 0; h < HT; ++h)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float unit = f[h][e] * k_unit;
-          float a = s[h][e], b = s[h][e + 2];
-          if (p.cap_out > 0.f) {
-            a = fmaf(tanhf(a * (unit * p.cap_in)), p.cap_out, ev);
-            b = fmaf(tanhf(b * (unit * p.cap_in)), p.cap_out, ev);
-          } else {
-            a = fmaf(a, unit * p.scale_log2, ev);
-            b = fmaf(b, unit * p.scale_log2, ev);
-          }
-          a = in0 ? a : -INFINITY;
-          b = in1 ? b : -INFINITY;
-          s[h][e] = a;
-          s[h][e + 2] = b;
-          float x = fmaxf(a, b);
+          float x = mx[h][e];
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -322,141 +347,179 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) attention_decode_kv8_kern
             for (int c = 0; c < NC; ++c) { o[h][c][e] *= by; o[h][c][e + 2] *= by; }
           }
       }
+    };
+    auto sees = [&](int kp) { return (kp >= lo || kp < keep) && kp <= pos; };
+    // score -> base 2 with the value scale's power; `unit`: what a unit of s is worth, times the softmax scale
+    auto scaled = [&](float s, float unit, float cap_unit, float ev) {
+      return p.cap_out > 0.f ? fmaf(tanhf(s * cap_unit), p.cap_out, ev) : fmaf(s, unit, ev);
+    };
+
+    if (tail_any) {
+      // the own block, in bfloat16 (its queries too)
+      uint32_t tv[NC][4];                                   // value words of positions 2j, 2j + 1, 2j + 8, 2j + 9: zeros where masked
+      bool in[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) in[r] = sees(tail0 + 2 * j + (r & 1) + (r >> 1) * 8);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          tv[c][r] = in[r] ? *reinterpret_cast<const uint32_t*>(vt_tail + (2 * j + (r & 1) + (r >> 1) * 8) * D + c * 16 + 2 * g) : 0u;
+      float s[HT][4] = {}, mx[HT][2];
+#pragma unroll
+      for (int c = 0; c < NC; c += 2) {
+        // a lane's 16 bytes of a row fill its places in two steps of k
+        const uint4 x = tk[c], y = tk[c + 1];
+        const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+#pragma unroll
+        for (int h = 0; h < HT; ++h) {
+          const uint4 b = h * 8 + g < G ? *reinterpret_cast<const uint4*>(q + (size_t)(h * 8 + g) * D + c * 16 + 8 * j)
+                                        : make_uint4(0u, 0u, 0u, 0u);
+          mma_bf16(s[h], a0, b.x, b.y);
+          mma_bf16(s[h], a1, b.z, b.w);
+        }
+      }
+      const bool in0 = sees(tail0 + g), in1 = sees(tail0 + g + 8);
 #pragma unroll
       for (int h = 0; h < HT; ++h)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          s[h][e] = ex2(s[h][e] - (m[h][e] - kLift));
-          s[h][e + 2] = ex2(s[h][e + 2] - (m[h][e] - kLift));
-          l[h][e] = fmaf(s[h][e] + s[h][e + 2], v_inv, l[h][e]);
+          s[h][e] = in0 ? scaled(s[h][e], p.scale_log2, p.cap_in, 0.f) : -INFINITY;
+          s[h][e + 2] = in1 ? scaled(s[h][e + 2], p.scale_log2, p.cap_in, 0.f) : -INFINITY;
+          mx[h][e] = fmaxf(s[h][e], s[h][e + 2]);
         }
-    };
-
-    if (has_tail) {
-      // the own block, in bfloat16: 16 positions per warp, from memory
-      const int first = own * PAGE + key0;
-      const bool any = first <= pos && (first + 15 >= lo || first < keep);
-      if (any) {
-        const size_t tail = ((size_t)slot * p.n_kv_heads + kvh) * (PAGE * D);
-        const __nv_bfloat16 *kt = p.k_tail + tail + key0 * D, *vt = p.v_tail + tail + key0 * D;
-        float s[HT][4] = {};
+      raise(mx);
+      uint32_t b[HT][2];
 #pragma unroll
-        for (int c = 0; c < NC; c += 2) {
-          // a lane's 16 bytes of a row fill its places in two steps of k
-          const uint4 x = *reinterpret_cast<const uint4*>(kt + g * D + c * 16 + 8 * j);
-          const uint4 y = *reinterpret_cast<const uint4*>(kt + (g + 8) * D + c * 16 + 8 * j);
-          const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+      for (int h = 0; h < HT; ++h) {
 #pragma unroll
-          for (int h = 0; h < HT; ++h) {
-            const uint4 b = h * 8 + g < G ? *reinterpret_cast<const uint4*>(q + (size_t)(h * 8 + g) * D + c * 16 + 8 * j)
-                                          : make_uint4(0u, 0u, 0u, 0u);
-            mma_bf16(s[h], a0, b.x, b.y);
-            mma_bf16(s[h], a1, b.z, b.w);
-          }
+        for (int e = 0; e < 4; ++e) {
+          s[h][e] = ex2(s[h][e] - (m[h][e & 1] - kLift));
+          l[h][e & 1] += s[h][e];
         }
-        // (these queries are whole: undo q's power)
-        float keep_f[HT][2];
+        b[h][0] = transposed(pack_bf16(s[h][0], s[h][1]));
+        b[h][1] = transposed(pack_bf16(s[h][2], s[h][3]));
+      }
 #pragma unroll
-        for (int h = 0; h < HT; ++h)
+      for (int c = 0; c < NC; ++c) {
+        const uint32_t a[4] = {__byte_perm(tv[c][0], tv[c][1], 0x5410), __byte_perm(tv[c][0], tv[c][1], 0x7632),
+                               __byte_perm(tv[c][2], tv[c][3], 0x5410), __byte_perm(tv[c][2], tv[c][3], 0x7632)};
 #pragma unroll
-          for (int e = 0; e < 2; ++e) { keep_f[h][e] = f[h][e]; f[h][e] = 1.f; }
-        softmax(s, first, true, 1.f, 0.f, 1.f);
-#pragma unroll
-        for (int h = 0; h < HT; ++h)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) f[h][e] = keep_f[h][e];
-        uint32_t b[HT][2];
-#pragma unroll
-        for (int h = 0; h < HT; ++h) {
-          b[h][0] = transposed(pack_bf16(s[h][0], s[h][1]));
-          b[h][1] = transposed(pack_bf16(s[h][2], s[h][3]));
-        }
-        bool in[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int kp = first + 2 * j + (r & 1) + (r >> 1) * 8;
-          in[r] = (kp >= lo || kp < keep) && kp <= pos;
-        }
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          uint32_t w[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            w[r] = in[r] ? *reinterpret_cast<const uint32_t*>(vt + (2 * j + (r & 1) + (r >> 1) * 8) * D + c * 16 + 2 * g) : 0u;
-          const uint32_t a[4] = {__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x5410),
-                                 __byte_perm(w[2], w[3], 0x7632)};
-#pragma unroll
-          for (int h = 0; h < HT; ++h) mma_bf16(o[h][c], a, b[h][0], b[h][1]);
-        }
+        for (int h = 0; h < HT; ++h) mma_bf16(o[h][c], a, b[h][0], b[h][1]);
       }
     }
 
-    const uint32_t ring_u = smem_u32(ring);
     float ks_all = 0.f, vs_all = 0.f;
-    for (int i = begin; i < end; ++i) {
-      const int n = i - begin, st = n % STAGES;
-      if ((n & 31) == 0) {                                  // scales of the next 32 items, one per lane
-        const int at = i + lane;
-        int page = at < end ? table[block_of(at)] : -1;
+    int at = 0;                                             // the slot of the next tile
+    uint32_t parity = 0;
+    auto next = [&] { if (++at == SLOTS) { at = 0; parity ^= 1u; } };
+    for (int x = 0; x < mine; ++x) {
+      if (x % 32 == 0) {                                    // scales of the next 32 of its half pages, one per lane
+        const int page = x + lane < mine ? table[block_at(x + lane)] : -1;
         const bool ok = page >= 0 && page < total_pages;
         ks_all = ok ? p.k_scale[(size_t)page * p.n_kv_heads + kvh] : 0.f;
         vs_all = ok ? p.v_scale[(size_t)page * p.n_kv_heads + kvh] : 1.f;
       }
-      const float ks = __shfl_sync(0xffffffffu, ks_all, n & 31), vs = __shfl_sync(0xffffffffu, vs_all, n & 31);
+      const float ks = __shfl_sync(0xffffffffu, ks_all, x & 31), vs = __shfl_sync(0xffffffffu, vs_all, x & 31);
       const int ev_i = (int)((__float_as_uint(vs) >> 23) & 0xffu) - 127;                  // vs = 2^ev_i
-      if (!mbar_wait(&full_bar[st], (n / STAGES) & 1, aborted)) break;
-      __syncwarp();
-      const int first = block_of(i) * PAGE + key0;
-      const bool ragged = first < lo && first + 15 >= keep;                 // (every position of a complete block is before pos)
-      const uint32_t kt = ring_u + st * 2 * S::TILE, vt = kt + S::TILE;
-      if (ragged) {
-        // value rows that the query does not see become zeros (e4m3 may hold a NaN there): two lanes a row
-        const int row = key0 + (lane >> 1), kp = block_of(i) * PAGE + row;
-        if (kp < lo && kp >= keep) {
+      const int first = block_at(x) * PAGE + (half_of(x) & 1) * POS;
+      const bool ragged = first < lo && first + POS - 1 >= keep;            // (every position of a complete block is before pos)
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars[at], parity, aborted))) break;
+      const uint32_t kt = smem_u32(slots + at * S::TILE);
+      float s[HT][MT][4] = {};
+      uint32_t w[2][MT][4];                                 // two chunks of every tile of positions; the next two are loaded meanwhile
+      auto load_k = [&](int c) {                            // positions 0-7 and 8-15 of a tile, chunk c, then chunk c + 1
 #pragma unroll
-          for (int c = 0; c < NC / 2; ++c)
-            *reinterpret_cast<uint4*>(ring + st * 2 * S::TILE + S::TILE + chunk_at<D>(row, (lane & 1) * (NC / 2) + c)) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        __syncwarp();
-      }
-      float s[HT][4] = {};
+        for (int mt = 0; mt < MT; ++mt) ldmatrix_x4(w[c >> 1 & 1][mt], kt + chunk_at<D>(mt * 16 + (lane & 15), c + (lane >> 4)));
+      };
+      load_k(0);
 #pragma unroll
       for (int c = 0; c < NC; c += 2) {
-        uint32_t w[4];                                      // positions 0-7 and 8-15 of chunk c, then of chunk c + 1
-        ldmatrix_x4(w, kt + chunk_at<D>(key0 + (lane & 15), c + (lane >> 4)));
+        if (c + 2 < NC) load_k(c + 2);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t a[4];
-          numbers<FMT, false>(w[2 * u], a[0], a[2]);
-          numbers<FMT, false>(w[2 * u + 1], a[1], a[3]);
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int h = 0; h < HT; ++h) mma_f16(s[h], a, qf[h][c + u][0], qf[h][c + u][1]);
-        }
+          for (int mt = 0; mt < MT; ++mt) {
+            uint32_t a[4];
+            numbers<FMT, false>(w[c >> 1 & 1][mt][2 * u], a[0], a[2]);
+            numbers<FMT, false>(w[c >> 1 & 1][mt][2 * u + 1], a[1], a[3]);
+#pragma unroll
+            for (int h = 0; h < HT; ++h) mma_f16(s[h][mt], a, qf[h][c + u][0], qf[h][c + u][1]);
+          }
       }
-      softmax(s, first, ragged, ks, (float)ev_i, kv8::power_of_two(-ev_i));
-      uint32_t b[HT][2];
+      __syncwarp();                                         // every lane has its keys (they are in products): the slot is free
+      ask(2 * x + SLOTS, at);
+      next();
+      const float ev = (float)ev_i, v_inv = kv8::power_of_two(-ev_i);
+      float mx[HT][2];
+#pragma unroll
+      for (int h = 0; h < HT; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float unit = f[h][e] * ks * p.scale_log2, cap_unit = f[h][e] * ks * p.cap_in;
+          float top = -INFINITY;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              float y = scaled(s[h][mt][e + 2 * r], unit, cap_unit, ev);
+              if (ragged && !sees(first + mt * 16 + g + 8 * r)) y = -INFINITY;
+              s[h][mt][e + 2 * r] = y;
+              top = fmaxf(top, y);
+            }
+          mx[h][e] = top;
+        }
+      raise(mx);
+      uint32_t b[HT][MT][2];
 #pragma unroll
       for (int h = 0; h < HT; ++h) {
-        b[h][0] = transposed(pack_f16(s[h][0], s[h][1]));
-        b[h][1] = transposed(pack_f16(s[h][2], s[h][3]));
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[h][mt][e] = ex2(s[h][mt][e] - (m[h][e & 1] - kLift));
+            sum[e & 1] += s[h][mt][e];
+          }
+          b[h][mt][0] = transposed(pack_f16(s[h][mt][0], s[h][mt][1]));
+          b[h][mt][1] = transposed(pack_f16(s[h][mt][2], s[h][mt][3]));
+        }
+        l[h][0] = fmaf(sum[0], v_inv, l[h][0]);
+        l[h][1] = fmaf(sum[1], v_inv, l[h][1]);
       }
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars[at], parity, aborted))) break;
+      const uint32_t vt = smem_u32(slots + at * S::TILE);
+      if (ragged) {
+        // value rows that the query does not see become zeros (e4m3 may hold a NaN there): a row a lane
+#pragma unroll 1
+        for (int c = 0; c < NC; ++c)
+          if (!sees(first + lane)) *reinterpret_cast<uint4*>(slots + at * S::TILE + chunk_at<D>(lane, c)) = make_uint4(0u, 0u, 0u, 0u);
+        __syncwarp();
+      }
+      auto load_v = [&](int c) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) ldmatrix_x4_trans(w[c >> 1 & 1][mt], vt + chunk_at<D>(mt * 16 + (lane & 15), c + (lane >> 4)));
+      };
+      load_v(0);
 #pragma unroll
       for (int c = 0; c < NC; c += 2) {
-        uint32_t w[4];
-        ldmatrix_x4_trans(w, vt + chunk_at<D>(key0 + (lane & 15), c + (lane >> 4)));
+        if (c + 2 < NC) load_v(c + 2);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t a[4];
-          numbers<FMT, true>(w[2 * u], a[0], a[1]);
-          numbers<FMT, true>(w[2 * u + 1], a[2], a[3]);
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int h = 0; h < HT; ++h) mma_f16(o[h][c + u], a, b[h][0], b[h][1]);
-        }
+          for (int u = 0; u < 2; ++u) {
+            uint32_t a[4];
+            numbers<FMT, true>(w[c >> 1 & 1][mt][2 * u], a[0], a[1]);
+            numbers<FMT, true>(w[c >> 1 & 1][mt][2 * u + 1], a[2], a[3]);
+#pragma unroll
+            for (int h = 0; h < HT; ++h) mma_f16(o[h][c + u], a, b[h][mt][0], b[h][mt][1]);
+          }
       }
-      // the zeros written above must be ordered before the copy engine writes this stage again
+      // the zeros written above must be ordered before the copy engine writes this slot again
       if (ragged) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty_bar[st]);
+      ask(2 * x + 1 + SLOTS, at);
+      next();
     }
     // l is a sum over this lane's positions: complete it over the lanes with the same heads
 #pragma unroll
@@ -467,8 +530,8 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) attention_decode_kv8_kern
         l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], 8);
         l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], 16);
       }
-    // every warp is done with the ring; all of them go on, or none (whatever the producer sets meanwhile)
-    if (!any_consumer(*aborted != 0)) {
+    // every warp is done with its slots; all of them go on, or none
+    if (!__syncthreads_or(*aborted)) {
       float* mo = reinterpret_cast<float*>(ring);           // [warps][heads][D]
 #pragma unroll
       for (int h = 0; h < HT; ++h) {
@@ -481,56 +544,53 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) attention_decode_kv8_kern
 #pragma unroll
           for (int e = 0; e < 2; ++e) { wm[warp][h * 8 + 2 * j + e] = m[h][e]; wl[warp][h * 8 + 2 * j + e] = l[h][e]; }
       }
-      consumers_sync();
-      for (int idx = tid; idx < G * D; idx += 32 * CONSUMERS) {
-        const int h = idx / D, d = idx % D, head = kvh * G + h;
-        float M = -1e30f, L = 0.f, acc = 0.f;
+      __syncthreads();
+      if (tid < G) {                                        // a thread per head: the warps' weights (in wm), the sum (in wl[0])
+        const int head = kvh * G + tid;
+        float M = -1e30f, L = 0.f;
 #pragma unroll
-        for (int w = 0; w < CONSUMERS; ++w) M = fmaxf(M, wm[w][h]);
+        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, wm[w][tid]);
 #pragma unroll
-        for (int w = 0; w < CONSUMERS; ++w) {
-          const float by = exp2f(wm[w][h] - M);
-          L += by * wl[w][h];
-          acc += by * mo[(size_t)(w * HT * 8 + h) * D + d];
+        for (int w = 0; w < WARPS; ++w) {
+          const float by = exp2f(wm[w][tid] - M);
+          L += by * wl[w][tid];
+          wm[w][tid] = by;
         }
         if (p.n_splits == 1) {
           L += sink_term(p.sink, head, M);
-          p.out[((size_t)t * p.n_heads + head) * D + d] = __float2bfloat16_rn(L == 0.f ? 0.f : acc / L);
+          wl[0][tid] = L == 0.f ? 0.f : 1.f / L;
         } else {
-          const size_t at = ((size_t)t * p.n_heads + head) * p.n_splits + split;
-          p.part_o[at * D + d] = acc;
-          if (d == 0) p.part_ml[at] = make_float2(M, L);
+          p.part_ml[((size_t)t * p.n_heads + head) * p.n_splits + split] = make_float2(M, L);
         }
       }
-      if (has_tail && pos % PAGE == PAGE - 1) {
-        // the block is complete: its codes and scales, for later steps
-        const int page = table[own];
-        if (page >= 0 && page < total_pages) {
-          const size_t tail = ((size_t)slot * p.n_kv_heads + kvh) * (PAGE * D), tile = ((size_t)page * p.n_kv_heads + kvh) * (PAGE * D);
-          constexpr int PER = PAGE * D / 8 / (32 * CONSUMERS);
-#pragma unroll 1
-          for (int which = 0; which < 2; ++which) {
-            const uint4* src = reinterpret_cast<const uint4*>((which ? p.v_tail : p.k_tail) + tail);
-            uint4 v[PER];
-            uint32_t top = 0;
+      __syncthreads();
+      for (int idx = tid; idx < G * D / 2; idx += NT) {
+        const int h = idx / (D / 2), d = idx % (D / 2) * 2, head = kvh * G + h;
+        float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) { v[i] = src[tid + i * 32 * CONSUMERS]; top = max(top, kv8::top_of(v[i])); }
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) top_s[which][warp] = top;
-            consumers_sync();
-#pragma unroll
-            for (int w = 0; w < CONSUMERS; ++w) top = max(top, top_s[which][w]);
-            const int e = kv8::scale_exponent<FMT>(__uint_as_float(top << 16));
-            const float inv = kv8::power_of_two(-e);
-            uint2* dst = reinterpret_cast<uint2*>((which ? p.v : p.k) + tile);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) dst[tid + i * 32 * CONSUMERS] = kv8::codes8<FMT>(v[i], inv);
-            if (tid == 0) (which ? p.v_scale_w : p.k_scale_w)[(size_t)page * p.n_kv_heads + kvh] = kv8::power_of_two(e);
-          }
-        } else if (tid == 0 && p.error_flag) {
-          atomicExch(p.error_flag, 3);
+        for (int w = 0; w < WARPS; ++w) {
+          const float2 x = *reinterpret_cast<const float2*>(mo + (size_t)(w * HT * 8 + h) * D + d);
+          const float by = wm[w][h];
+          acc.x = fmaf(by, x.x, acc.x);
+          acc.y = fmaf(by, x.y, acc.y);
+        }
+        if (p.n_splits == 1) {
+          const float inv = wl[0][h];
+          *reinterpret_cast<uint32_t*>(p.out + ((size_t)t * p.n_heads + head) * D + d) = pack_bf16(acc.x * inv, acc.y * inv);
+        } else {
+          *reinterpret_cast<float2*>(p.part_o + (((size_t)t * p.n_heads + head) * p.n_splits + split) * D + d) = acc;
         }
       }
+    }
+  }
+  if (has_tail && pos % PAGE == PAGE - 1) {
+    // the block is complete: its codes and scales, for later steps (nobody reads that page in this one)
+    const int page = table[own];
+    if (page >= 0 && page < total_pages) {
+      const size_t to = (size_t)page * p.n_kv_heads + kvh;
+      hold_tail<D, FMT, NT>(p.k_tail + tail, p.v_tail + tail, p.k + to * (PAGE * D), p.v + to * (PAGE * D), p.k_scale_w + to, p.v_scale_w + to, top_s);
+    } else if (tid == 0 && p.error_flag) {
+      atomicExch(p.error_flag, 3);
     }
   }
   if (*aborted) {
@@ -602,8 +662,8 @@ __global__ void __launch_bounds__(D) attention_decode_kv8_combine(const float* _
 template <int D, int FMT, int HT>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int n_tokens, cudaStream_t stream) {
   auto* kernel = attention_decode_kv8_kernel<D, FMT, HT>;
-  constexpr int MERGE = CONSUMERS * HT * 8 * D * 4;
-  constexpr int SMEM = (Shape<D>::RING > MERGE ? Shape<D>::RING : MERGE) + 1024;
+  using S = Shape<D, HT>;
+  constexpr int SMEM = S::SMEM;
   static bool ready[64] = {};                               // per device
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !ready[dev]) {
@@ -615,7 +675,7 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int n_
     }
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
-  cpi::launch_pdl(kernel, dim3(p.n_splits, p.n_kv_heads, n_tokens), NT, SMEM, stream, mk, mv, p);
+  cpi::launch_pdl(kernel, dim3(p.n_splits, p.n_kv_heads, n_tokens), S::NT, SMEM, stream, mk, mv, p);
   if (check_launch("attention_decode_kv8")) return 2;
   if (p.n_splits > 1) {
     cpi::launch_pdl(attention_decode_kv8_combine<D>, n_tokens * p.n_heads, D, 0, stream, p.part_o, p.part_ml, p.out, p.n_splits, p.sink,
@@ -636,7 +696,7 @@ extern "C" int cpi_attention_decode_kv8_supported(int n_heads, int n_kv_heads, i
 }
 
 // Blocks of threads that share an SM, for the caller's choice of `n_splits`.
-extern "C" int cpi_attention_decode_kv8_blocks_per_sm(int group) { return group <= 8 ? 3 : 2; }
+extern "C" int cpi_attention_decode_kv8_blocks_per_sm(int head_dim) { return head_dim ? 2 : 2; }
 
 // q, out [T, NH, D] bfloat16, one token per sequence; codes k, v [n_pages, NKV, 64, D]; `fmt` 0 int8, 1 e4m3.  `scratch`:
 // T * NH * splits * (D + 2) floats, 8-byte aligned (unused when n_splits == 1).
@@ -653,12 +713,12 @@ extern "C" int cpi_attention_decode_kv8(const void* q, void* out, void* k, void*
   CPI_REQUIRE(n_splits >= 1 && n_splits <= dec8::kMaxSplits && n_tokens <= 65535, "attention_decode_kv8: bad grid (%d splits of at most %d, %d tokens)",
               n_splits, dec8::kMaxSplits, n_tokens);
   CPI_REQUIRE(n_splits == 1 || scratch, "attention_decode_kv8: split scratch is missing");
-  // the codes as lines of 128 bytes: a (page, head) tile is 64 * D / 128 of them
+  // the codes as lines of 128 bytes: a tile of 32 positions of a head is 32 * D / 128 of them
   CUtensorMap mk, mv;
   const uint64_t lines = (uint64_t)n_pages * n_kv_heads * (kv8::PAGE * head_dim / 128);
   CPI_REQUIRE(n_pages > 0 && lines + kv8::PAGE < (1ull << 31), "attention_decode_kv8: a cache of %d pages of %d heads", n_pages, n_kv_heads);
-  if (tc::get_map_2d_bf16(k, 64, lines, 128, 64, kv8::PAGE * head_dim / 128, &mk)) return 1;
-  if (tc::get_map_2d_bf16(v, 64, lines, 128, 64, kv8::PAGE * head_dim / 128, &mv)) return 1;
+  if (tc::get_map_2d_bf16(k, 64, lines, 128, 64, 32 * head_dim / 128, &mk)) return 1;
+  if (tc::get_map_2d_bf16(v, 64, lines, 128, 64, 32 * head_dim / 128, &mv)) return 1;
   const long parts = (long)n_tokens * n_heads * n_splits;
   dec8::Params p{(const __nv_bfloat16*)q, (__nv_bfloat16*)out, k_scale, v_scale, (const __nv_bfloat16*)k_tail, (const __nv_bfloat16*)v_tail,
                  (uint8_t*)k, (uint8_t*)v, k_scale, v_scale, page_table, max_blocks, n_pages, n_slots, n_seqs, token_seq, token_pos, seq_slot,

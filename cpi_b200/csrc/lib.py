@@ -1208,7 +1208,7 @@ def attention_decode_kv8(q, out, cache, page_table, token_seq, token_pos, seq_sl
     longest = min(int(max_context), table[1] * 64)
     if window_kind != WINDOW_FULL:
         longest = min(longest, window_size + 64 + -(-keep_first // 64) * 64)
-    splits = _kv8_splits(here, T * nkv, -(-max(longest, 1) // 64), n_heads // nkv)
+    splits = _kv8_splits(here, T * nkv, -(-max(longest, 1) // 64), d)
     scratch = None if splits == 1 else torch.empty(T * n_heads * splits * (d + 2), dtype=torch.float32, device=q.device)
     _run(_declared("cpi_attention_decode_kv8", "ppppppippipipppiiiiiiiiiffpippp"),
          q.data_ptr(), out.data_ptr(), at[0], at[1], at[2], at[3], cache.k.shape[0], at[4], at[5], k_tail.shape[0], page_table.data_ptr(), table[1],
@@ -1218,9 +1218,9 @@ def attention_decode_kv8(q, out, cache, page_table, token_seq, token_pos, seq_sl
 
 
 @functools.lru_cache(maxsize=4096)
-def _kv8_splits(device: int, base: int, pages: int, group: int) -> int:
+def _kv8_splits(device: int, base: int, pages: int, head_dim: int) -> int:
     """Blocks of threads that share a sequence's keys, for `base` (token, kv head) pairs of up to `pages` pages each."""
-    slots = load().cpi_attention_decode_kv8_blocks_per_sm(c_int(group)) * sm_count()
+    slots = load().cpi_attention_decode_kv8_blocks_per_sm(c_int(head_dim)) * sm_count()
     want = slots // base if base <= slots else -(-4 * slots // base)
     return max(1, min(want, (pages + 1) // 4, MAX_DECODE_SPLITS))
 

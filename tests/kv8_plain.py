@@ -88,12 +88,29 @@ def attend(q, k, v, positions, *, fmt, scale, window="full", size=0, keep=0, sin
             s = torch.cat([s, sink.double()[:, None]], 1)
         p = torch.softmax(s, 1)[:, :len(at)]
         out[i] = torch.einsum("hj,jhd->hd", p, vv)
-        mag[i] = torch.einsum("hj,jhd->hd", p, vv.abs())
+        mag[i] = torch.einsum("hj,jhd->hd", p, vv.abs()) + 2.0 ** 8 * floor(p, at, hv, pos // BLOCK * BLOCK, nh // nkv)
     return out, mag
+
+
+def floor(p, at, held, edge, group):
+    """What the float16 probabilities of single tokens may be off by whatever their size, as an output [heads, 1].  A kernel
+    multiplies a block's codes c by float16 numbers P = p 2^e x (2^e the block's scale, x the same for all), the largest of which
+    is 2^6 or more; float16 numbers are at most 2^-25 from what they round (half the step of its smallest ones), so a term is off
+    by 2^-25 |c| beside a largest P of 2^6: by 2^-31 |c| max(p 2^e).  |c| is below 2^9, and max(p 2^e) |c| at most 2^2 times
+    max(p m), m the largest held number of p's block, for |c| <= 2^8 m / 2^e / 2^6: int8 codes reach 64 or more, e4m3 codes 128."""
+    m = torch.zeros_like(p)
+    far = at < edge
+    if not far.any():
+        return torch.zeros(p.shape[0], 1, dtype=p.dtype, device=p.device)
+    blocks = at // BLOCK
+    for b in blocks[far].unique().tolist():
+        top = held[b * BLOCK:(b + 1) * BLOCK].abs().amax((0, 2)).repeat_interleave(group)          # per head
+        m[:, blocks == b] = top[:, None]
+    return int(far.sum()) * 2.0 ** -31 * 2.0 ** 2 * (p * m * far).amax(1, keepdim=True)
 
 
 def tolerance(out, mag):
     """The output is rounded to bfloat16 (2^-8 of its value); probabilities are rounded to bfloat16 or finer before they are
-    multiplied (2^-8 of each term's size, so of their sum); scores, exponentials and sums are float32 (2^-10 of the terms' size
+    multiplied (2^-8 of each term's size, so of their sum; `floor` below that); scores, exponentials and sums are float32 (2^-10 of the terms' size
     covers scores up to 1,000)."""
     return 2.0 ** -8 * out.abs() + (2.0 ** -8 + 2.0 ** -10) * mag + 1e-30
