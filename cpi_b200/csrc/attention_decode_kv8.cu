@@ -43,6 +43,7 @@ constexpr uint32_t kSpinLimit = 1u << 24;
 constexpr float kSlack = 8.f, kLift = 6.f;        // p = 2^(s + e - m + kLift), m raised when s + e exceeds it by kSlack
 constexpr int kTailUnits = 2;                     // a tail's bytes, in pages of codes
 constexpr int kMaxSplits = 256;
+constexpr int kMaxCluster = 8;                    // splits that are joined over distributed shared memory
 
 struct Params {
   const __nv_bfloat16* q; __nv_bfloat16* out;     // [T, NH, D]
@@ -55,6 +56,7 @@ struct Params {
   int window_kind, window_size, keep_first;
   float scale_log2, cap_in, cap_out;              // soft cap c > 0: scale / c and c log2(e); else 0
   int n_splits;
+  bool clustered;                                 // the splits of a (token, key/value head) are a cluster
   float* part_o; float2* part_ml;                 // [T, NH, splits, D], [T, NH, splits]
   const float* sink;
   int* error_flag;
@@ -131,6 +133,21 @@ __device__ __forceinline__ int window_low(int kind, int size, int pos) {
 __device__ __forceinline__ float sink_term(const float* sink, int head, float m) {
   return sink ? exp2f(fminf(sink[head] * 1.4426950408889634f - m + kLift, 120.f)) : 0.f;
 }
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Two floats at the place of `at` (an address in this block's shared memory) in block `rank` of the cluster.
+__device__ __forceinline__ float2 peer_pair(uint32_t at, uint32_t rank) {
+  float2 v;
+  asm volatile("{\n\t.reg .u32 r;\n\tmapa.shared::cluster.u32 r, %2, %3;\n\tld.shared::cluster.v2.f32 {%0, %1}, [r];\n\t}"
+               : "=f"(v.x), "=f"(v.y) : "r"(at), "r"(rank) : "memory");
+  return v;
+}
 // The four codes of a word as two pairs of float16: bytes (0, 1) and (2, 3), or with SPLIT bytes (0, 2) and (1, 3).
 template <int FMT, bool SPLIT> __device__ __forceinline__ void numbers(uint32_t w, uint32_t& a, uint32_t& b) {
   if (FMT == kv8::kInt8) {
@@ -201,8 +218,11 @@ __global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kern
   __shared__ uint64_t full_bar[WARPS * SLOTS];
   __shared__ float wm[WARPS][HT * 8], wl[WARPS][HT * 8];
   __shared__ uint32_t top_s[16];
+  __shared__ float2 ml_s[HT * 8];                           // this split's reference and sum per head, for the cluster
   __shared__ int abort_s;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  float* sums = reinterpret_cast<float*>(ring + S::MERGE);  // [G][D]: this split's outputs, for the cluster
+  static_assert(S::RING >= S::MERGE + HT * 8 * D * 4, "room for the sums behind what the warps leave");
   const int split = blockIdx.x, kvh = blockIdx.y, t = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, j = lane & 3;
@@ -559,6 +579,8 @@ __global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kern
         if (p.n_splits == 1) {
           L += sink_term(p.sink, head, M);
           wl[0][tid] = L == 0.f ? 0.f : 1.f / L;
+        } else if (p.clustered) {
+          ml_s[tid] = make_float2(M, L);
         } else {
           p.part_ml[((size_t)t * p.n_heads + head) * p.n_splits + split] = make_float2(M, L);
         }
@@ -577,11 +599,44 @@ __global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kern
         if (p.n_splits == 1) {
           const float inv = wl[0][h];
           *reinterpret_cast<uint32_t*>(p.out + ((size_t)t * p.n_heads + head) * D + d) = pack_bf16(acc.x * inv, acc.y * inv);
+        } else if (p.clustered) {
+          *reinterpret_cast<float2*>(sums + h * D + d) = acc;
         } else {
           *reinterpret_cast<float2*>(p.part_o + (((size_t)t * p.n_heads + head) * p.n_splits + split) * D + d) = acc;
         }
       }
     }
+  }
+  if (p.clustered) {
+    // The splits' sums, each in its block's shared memory: every block joins a share of the outputs.  (All threads of all blocks
+    // pass both barriers, whatever has happened before.)
+    cluster_sync();
+    const int rank = (int)cluster_rank(), n = p.n_splits;
+    for (int i = rank + n * tid; i < G * D / 2; i += n * NT) {
+      const int h = i / (D / 2), d = i % (D / 2) * 2, head = kvh * G + h;
+      const uint32_t at = smem_u32(sums + h * D + d), ml_at = smem_u32(&ml_s[h]);
+      float2 ml[kMaxCluster], v[kMaxCluster];
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        ml[r] = r < n ? peer_pair(ml_at, r) : make_float2(-1e30f, 0.f);
+        v[r] = r < n ? peer_pair(at, r) : make_float2(0.f, 0.f);
+      }
+      float M = -1e30f, L = 0.f;
+      float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) M = fmaxf(M, ml[r].x);
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        const float by = exp2f(ml[r].x - M);
+        L += by * ml[r].y;
+        acc.x = fmaf(by, v[r].x, acc.x);
+        acc.y = fmaf(by, v[r].y, acc.y);
+      }
+      L += sink_term(p.sink, head, M);
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      *reinterpret_cast<uint32_t*>(p.out + ((size_t)t * p.n_heads + head) * D + d) = pack_bf16(acc.x * inv, acc.y * inv);
+    }
+    cluster_sync();                                         // nobody leaves while its shared memory is read
   }
   if (has_tail && pos % PAGE == PAGE - 1) {
     // the block is complete: its codes and scales, for later steps (nobody reads that page in this one)
@@ -675,9 +730,23 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int n_
     }
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
-  cpi::launch_pdl(kernel, dim3(p.n_splits, p.n_kv_heads, n_tokens), S::NT, SMEM, stream, mk, mv, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.n_splits, p.n_kv_heads, n_tokens);
+  cfg.blockDim = dim3(S::NT);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.n_splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.clustered ? 2 : 1;
+  count_launch();
+  cudaLaunchKernelEx(&cfg, kernel, mk, mv, p);
   if (check_launch("attention_decode_kv8")) return 2;
-  if (p.n_splits > 1) {
+  if (p.n_splits > 1 && !p.clustered) {
     cpi::launch_pdl(attention_decode_kv8_combine<D>, n_tokens * p.n_heads, D, 0, stream, p.part_o, p.part_ml, p.out, p.n_splits, p.sink,
                     p.n_heads);
     return check_launch("attention_decode_kv8_combine");
@@ -695,11 +764,19 @@ extern "C" int cpi_attention_decode_kv8_supported(int n_heads, int n_kv_heads, i
   return (head_dim == 64 || head_dim == 128) && page_size == kv8::PAGE && n_heads / n_kv_heads <= 16 && n_kv_heads <= 65535;
 }
 
+// Whether `n_splits` blocks of threads for each of `base` (token, kv head) pairs are joined within the kernel, as clusters, or
+// through scratch by a second one.  A cluster saves a launch and the scratch, but its blocks stay until the last of them is
+// through: 160 blocks (5 windowed sequences, 8 kv heads of 64) take 7.3 us as clusters and 7.4 with the second kernel, 256 (8 x 4,096
+// positions, 8 kv heads of 128) 23.2 and 21.3, 1,536 (64 sequences) 201 and 188.
+extern "C" int cpi_attention_decode_kv8_clustered(int base, int n_splits) {
+  return n_splits > 1 && n_splits <= dec8::kMaxCluster && 3l * base * n_splits <= 4l * sm_count();
+}
+
 // Blocks of threads that share an SM, for the caller's choice of `n_splits`.
-extern "C" int cpi_attention_decode_kv8_blocks_per_sm(int head_dim) { return head_dim ? 2 : 2; }
+extern "C" int cpi_attention_decode_kv8_blocks_per_sm() { return 2; }
 
 // q, out [T, NH, D] bfloat16, one token per sequence; codes k, v [n_pages, NKV, 64, D]; `fmt` 0 int8, 1 e4m3.  `scratch`:
-// T * NH * splits * (D + 2) floats, 8-byte aligned (unused when n_splits == 1).
+// T * NH * splits * (D + 2) floats, 8-byte aligned (none if they are joined in the kernel).
 extern "C" int cpi_attention_decode_kv8(const void* q, void* out, void* k, void* v, float* k_scale, float* v_scale, int n_pages,
                                         const void* k_tail, const void* v_tail, int n_slots, const int* page_table, int max_blocks,
                                         const int* token_seq, const int* token_pos, const int* seq_slot, int n_seqs, int n_tokens, int n_heads,
@@ -712,7 +789,9 @@ extern "C" int cpi_attention_decode_kv8(const void* q, void* out, void* k, void*
   CPI_REQUIRE(window_kind == 0 || window_size > 0, "attention_decode_kv8: window kind %d needs a size > 0", window_kind);
   CPI_REQUIRE(n_splits >= 1 && n_splits <= dec8::kMaxSplits && n_tokens <= 65535, "attention_decode_kv8: bad grid (%d splits of at most %d, %d tokens)",
               n_splits, dec8::kMaxSplits, n_tokens);
-  CPI_REQUIRE(n_splits == 1 || scratch, "attention_decode_kv8: split scratch is missing");
+  // Without scratch the splits are joined in the kernel (see cpi_attention_decode_kv8_clustered).
+  const bool clustered = n_splits > 1 && !scratch;
+  CPI_REQUIRE(!clustered || n_splits <= dec8::kMaxCluster, "attention_decode_kv8: split scratch is missing");
   // the codes as lines of 128 bytes: a tile of 32 positions of a head is 32 * D / 128 of them
   CUtensorMap mk, mv;
   const uint64_t lines = (uint64_t)n_pages * n_kv_heads * (kv8::PAGE * head_dim / 128);
@@ -723,7 +802,7 @@ extern "C" int cpi_attention_decode_kv8(const void* q, void* out, void* k, void*
   dec8::Params p{(const __nv_bfloat16*)q, (__nv_bfloat16*)out, k_scale, v_scale, (const __nv_bfloat16*)k_tail, (const __nv_bfloat16*)v_tail,
                  (uint8_t*)k, (uint8_t*)v, k_scale, v_scale, page_table, max_blocks, n_pages, n_slots, n_seqs, token_seq, token_pos, seq_slot,
                  n_heads, n_kv_heads, window_kind, window_size, keep_first > 0 ? keep_first : 0, scale * 1.4426950408889634f,
-                 softcap > 0.f ? scale / softcap : 0.f, softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, n_splits,
+                 softcap > 0.f ? scale / softcap : 0.f, softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, n_splits, clustered,
                  scratch, scratch ? reinterpret_cast<float2*>(scratch + parts * head_dim) : nullptr, sink, error_flag};
   const bool wide = n_heads / n_kv_heads > 8;
 #define CPI_DEC8(D, F) (wide ? dec8::launch<D, F, 2>(mk, mv, p, n_tokens, stream) : dec8::launch<D, F, 1>(mk, mv, p, n_tokens, stream))

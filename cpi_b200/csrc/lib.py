@@ -1108,11 +1108,13 @@ def _run(fn, *args):
 
 def _here(what, *ts):
     """Kernels are launched on the current device's stream: all of a call's tensors have to be there.  Returns the device's number."""
-    here = torch._C._cuda_getDevice() if any(t.is_cuda for t in ts) else -1
+    here = ts[0].get_device()
     for t in ts:
         if t.get_device() != here or here < 0:
-            _need_cuda(t)
-            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{here}")
+            _need_cuda(*ts)
+            raise KernelError(f"{what}: tensors on {ts[0].device} and {t.device}")
+    if here != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: tensors on cuda:{here}, the current device is cuda:{torch._C._cuda_getDevice()}")
     return here
 
 
@@ -1208,8 +1210,8 @@ def attention_decode_kv8(q, out, cache, page_table, token_seq, token_pos, seq_sl
     longest = min(int(max_context), table[1] * 64)
     if window_kind != WINDOW_FULL:
         longest = min(longest, window_size + 64 + -(-keep_first // 64) * 64)
-    splits = _kv8_splits(here, T * nkv, -(-max(longest, 1) // 64), d)
-    scratch = None if splits == 1 else torch.empty(T * n_heads * splits * (d + 2), dtype=torch.float32, device=q.device)
+    splits, joined = _kv8_splits(here, T * nkv, -(-max(longest, 1) // 64))
+    scratch = torch.empty(T * n_heads * splits * (d + 2), dtype=torch.float32, device=q.device) if joined else None
     _run(_declared("cpi_attention_decode_kv8", "ppppppippipipppiiiiiiiiiffpippp"),
          q.data_ptr(), out.data_ptr(), at[0], at[1], at[2], at[3], cache.k.shape[0], at[4], at[5], k_tail.shape[0], page_table.data_ptr(), table[1],
          token_seq.data_ptr(), token_pos.data_ptr(), seq_slot.data_ptr(), seq_slot.numel(), T, n_heads, nkv, d, fmt, window_kind, int(window_size),
@@ -1218,11 +1220,13 @@ def attention_decode_kv8(q, out, cache, page_table, token_seq, token_pos, seq_sl
 
 
 @functools.lru_cache(maxsize=4096)
-def _kv8_splits(device: int, base: int, pages: int, head_dim: int) -> int:
-    """Blocks of threads that share a sequence's keys, for `base` (token, kv head) pairs of up to `pages` pages each."""
-    slots = load().cpi_attention_decode_kv8_blocks_per_sm(c_int(head_dim)) * sm_count()
+def _kv8_splits(device: int, base: int, pages: int):
+    """(Blocks of threads that share a sequence's keys, for `base` (token, kv head) pairs of up to `pages` pages each; whether a
+    second kernel joins them)."""
+    slots = load().cpi_attention_decode_kv8_blocks_per_sm() * sm_count()
     want = slots // base if base <= slots else -(-4 * slots // base)
-    return max(1, min(want, (pages + 1) // 4, MAX_DECODE_SPLITS))
+    n = max(1, min(want, (pages + 1) // 4, MAX_DECODE_SPLITS))
+    return n, n > 1 and not load().cpi_attention_decode_kv8_clustered(c_int(base), c_int(n))
 
 
 def kv8_stage(cache, page_table, plan, k_pages, v_pages):
