@@ -58,7 +58,7 @@ struct Params {
   int keep_first;                     // sliding window: a sequence's first positions stay visible to every later query
   float cap_in, cap_out;              // soft cap c > 0 on the scaled scores: cap_in = scale / c, cap_out = c log2(e); else 0
   const int* exact_table;             // BLOCKED: pages by sequence of the step and block (page_table: those of earlier blocks), -1 none
-  int n_pages;
+  int n_pages, n_tokens, n_seqs;
   int n_splits;                       // BLOCKED: blocks of threads that share a query tile's axis of key tiles
   float* part_o; float2* part_ml;     // with several: [T, NH, splits, D] sums, [T, NH, splits] reference and row sum
 };
@@ -111,10 +111,22 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
   pdl_launch_dependents();                              // (in this order, and not before the tensor memory is ours: see common.cuh)
   const int tile = blockIdx.y, head = blockIdx.x;       // heads are the fast axis: all heads of the longest tile start first
   const int kvh = head / (p.n_heads / p.n_kv_heads);
-  const int tok0 = p.tile_tok0[tile], rows = p.tile_rows[tile];
-  const int slot = BLOCKED ? p.token_seq[tok0] : p.seq_slot[p.token_seq[tok0]];
+  int tok0 = p.tile_tok0[tile], rows = p.tile_rows[tile];
+  if (BLOCKED) {                                        // indices outside of the step: somewhere within it, and the error flag
+    const bool good = tok0 >= 0 && tok0 < p.n_tokens && rows >= 1 && rows <= kTileRows && rows <= p.n_tokens - tok0;
+    tok0 = min(max(tok0, 0), p.n_tokens - 1);
+    rows = min(max(rows, 1), min(kTileRows, p.n_tokens - tok0));
+    if (!good && tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+  }
+  int slot = BLOCKED ? p.token_seq[tok0] : p.seq_slot[p.token_seq[tok0]];
   // the tile's rows are consecutive positions of one sequence; rows 0-127 are query tile A, the rest tile B
-  const int pos_first = p.token_pos[tok0], pos_last = pos_first + rows - 1;
+  int pos_first = p.token_pos[tok0];
+  if (BLOCKED && (slot < 0 || slot >= p.n_seqs || pos_first < 0 || pos_first > p.max_blocks * PAGE - rows)) {
+    slot = 0;
+    pos_first = 0;
+    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+  }
+  const int pos_last = pos_first + rows - 1;
   const int rows_x[2] = {min(rows, BQ), max(rows - BQ, 0)};
   const bool has_b = rows_x[1] > 0;
   const int p0_x[2] = {pos_first, pos_first + BQ};                         // first position of A, of B
@@ -639,7 +651,7 @@ extern "C" int cpi_attention_prefill(const void* q, void* out, const void* k_cac
   pre::Params p{(__nv_bfloat16*)out, page_table, max_blocks, token_pos, token_seq, seq_slot, tile_tok0, tile_rows,
                 n_heads, n_kv_heads, window_kind, window_size, scale * 1.4426950408889634f, error_flag, sink,
                 keep_first > 0 ? keep_first : 0, softcap > 0.f ? scale / softcap : 0.f,
-                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, nullptr, 0, 1, nullptr, nullptr};
+                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, nullptr, 0, 0, 0, 1, nullptr, nullptr};
   dim3 grid(n_heads, n_tiles);
   const int halves = head_dim / 64;
   const int smem = halves * 128 * 128 * (2 + pre::kRingSlots);     // Q of both tiles, the ring of K and V tiles
@@ -660,12 +672,12 @@ extern "C" int cpi_attention_prefill(const void* q, void* out, const void* k_cac
 // step and block by earlier_table and exact_table [sequences, width] (-1: none).  `n_splits` > 1: that many blocks of threads share a query tile's
 // keys, through `scratch` (n_tokens * n_heads * n_splits * (head_dim + 2) floats).
 extern "C" int cpi_attention_prefill_kv8(const void* q, void* out, const void* k_pages, const void* v_pages, long n_pages,
-                                         const int* earlier_table, const int* exact_table, int width, const int* token_seq,
+                                         const int* earlier_table, const int* exact_table, int n_seqs, int width, const int* token_seq,
                                          const int* token_pos, const int* tile_tok0, const int* tile_rows, int n_tiles, int n_tokens,
                                          int n_heads, int n_kv_heads, int head_dim, int window_kind, int window_size, int keep_first,
                                          float scale, float softcap, const float* sink, int n_splits, float* scratch, int* error_flag,
                                          cudaStream_t stream) {
-  if (n_tiles == 0) return 0;
+  if (n_tiles == 0 || n_tokens == 0) return 0;
   const long rows = (long)n_tokens * n_heads;
   CPI_REQUIRE(n_splits >= 1 && n_splits <= 32 && (n_splits == 1 || scratch), "attention_prefill_kv8: %d shares (up to 32, with scratch)", n_splits);
   CPI_REQUIRE(cpi_attention_prefill_supported(n_heads, n_kv_heads, head_dim, pre::PAGE),
@@ -682,10 +694,13 @@ extern "C" int cpi_attention_prefill_kv8(const void* q, void* out, const void* k
   pre::Params p{(__nv_bfloat16*)out, earlier_table, width, token_pos, token_seq, nullptr, tile_tok0, tile_rows,
                 n_heads, n_kv_heads, window_kind, window_size, scale * 1.4426950408889634f, error_flag, sink,
                 keep_first > 0 ? keep_first : 0, softcap > 0.f ? scale / softcap : 0.f,
-                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, exact_table, (int)n_pages, n_splits, scratch,
+                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, exact_table, (int)n_pages, n_tokens, n_seqs, n_splits, scratch,
                 scratch ? reinterpret_cast<float2*>(scratch + rows * n_splits * head_dim) : nullptr};
   dim3 grid(n_heads, n_tiles, n_splits);
-  const int smem = head_dim / 64 * 128 * 128 * (2 + pre::kRingSlots);
+  // One block of threads to an SM: each takes all of the tensor memory.  Two heads' worth of 64 would fit an SM's shared memory, and
+  // a second block that is put there, while the kernel before still fills the other SMs, waits for the first to end (four windowed
+  // prompts, 144 blocks: 80 us instead of 47).
+  const int smem = head_dim == 64 ? 120 * 1024 : head_dim / 64 * 128 * 128 * (2 + pre::kRingSlots);
   auto launch = [&](auto dim, auto capped) {
     auto* kernel = pre::attention_prefill_kernel<dim.value, capped.value, true>;
     static bool set[64] = {};                              // per device

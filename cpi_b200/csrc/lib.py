@@ -1161,8 +1161,10 @@ def _bf16_rows(what, shape, *ts):
 def _attention_options(what, n_heads, scale, window_kind, window_size, keep_first, sink, softcap):
     if window_kind not in (WINDOW_FULL, WINDOW_CHUNK, WINDOW_SLIDING) or (window_kind != WINDOW_FULL and window_size < 1):
         raise KernelError(f"{what}: window kind {window_kind} of size {window_size}")
-    if keep_first < 0 or not scale > 0 or softcap is not None and softcap < 0:
+    if keep_first < 0 or not scale > 0 or softcap is not None and not softcap >= 0:
         raise KernelError(f"{what}: keep_first {keep_first}, scale {scale}, softcap {softcap}")
+    if window_size > 1 << 30 or keep_first > 1 << 30:
+        raise KernelError(f"{what}: a window of {window_size} with {keep_first} kept positions (up to 2^30)")
     if sink is not None and (sink.dtype is not torch.float32 or not sink.is_contiguous() or sink.numel() != n_heads):
         raise KernelError(f"{what}: a sink is float32 [{n_heads}]")
 
@@ -1191,7 +1193,9 @@ def attention_decode_kv8(q, out, cache, page_table, token_seq, token_pos, seq_sl
     the tail's codes and scales are written to page page_table[slot, b].  `max_context`: no sequence is longer (it sizes the
     division of the keys over blocks of threads; any number is right, a good one is fast).  Windows, kept first positions,
     sink and soft cap as in `attention_decode`.  A token at a negative position is a padded row: its output is zero.  Tokens
-    of a call belong to different slots."""
+    of a call belong to different slots.  The index arrays and the page table are read before the kernels in front of this one
+    end: no kernel of this library may be writing them (copies and other kernels have ended by then).  An index outside
+    of the cache sets the error word (`device_error_flags`) and gives zeros; nothing is read or written for it."""
     what = "attention_decode_kv8"
     fmt, nkv, d, at = _kv8(cache, what, n_heads)
     T, k_tail = q.shape[0], cache.k_tail
@@ -1273,8 +1277,8 @@ def attention_prefill_kv8(q, out, k_pages, v_pages, plan, token_seq, token_pos, 
         raise KernelError(f"{what}: window kind {window_kind} of {window_size}, {keep_first} kept: the plan was made for {plan.window}")
     splits = _kv8_prefill_splits(here, tiles * n_heads, plan.most_tiles)
     scratch = None if splits == 1 else torch.empty(plan.n_tokens * n_heads * splits * (d + 2), dtype=torch.float32, device=q.device)
-    _run(_declared("cpi_attention_prefill_kv8", "pppplppippppiiiiiiiiffpippp"), q.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-         plan.n_pages, plan.earlier_table.data_ptr(), plan.exact_table.data_ptr(), plan.width, token_seq.data_ptr(), token_pos.data_ptr(),
+    _run(_declared("cpi_attention_prefill_kv8", "pppplppiippppiiiiiiiiffpippp"), q.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+         plan.n_pages, plan.earlier_table.data_ptr(), plan.exact_table.data_ptr(), plan.n_seqs, plan.width, token_seq.data_ptr(), token_pos.data_ptr(),
          tile_tok0.data_ptr(), tile_rows.data_ptr(), tiles, plan.n_tokens, n_heads, nkv, d, window_kind, int(window_size), int(keep_first), scale,
          softcap or 0.0, None if sink is None else sink.data_ptr(), splits, None if scratch is None else scratch.data_ptr(), _flag(here),
          _raw_stream(here))

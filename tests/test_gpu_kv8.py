@@ -236,6 +236,29 @@ def test_padded_rows_and_wrong_indices():
     rig.check(0, q[:1], out2[:1].view(1, 8, 128), [99])
 
 
+def test_prompt_indices_outside_of_the_step():
+    """Tiles, sequences and positions that the plan does not have: the error word, and nothing outside of the output is touched."""
+    rig = Rig([300, 200], seed=9)
+    flags = K.device_error_flags(DEV)
+    assert int(flags[0]) == 0
+    starts, news = [0, 0], [300, 200]
+    batch = rig.stager.stage(rig.slots, starts, [[0] * m for m in news], [[], []], torch.bfloat16)
+    plan = Kv8Plan(starts, news, rig.slots, device=DEV)
+    kp = torch.zeros(plan.n_pages, 2, 64, 128, dtype=torch.bfloat16, device=DEV)
+    vp, q = kp.clone(), rig.rows(500, 8 * 128)
+    store = torch.full((502, 8 * 128), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = store[1:501]
+    good = dict(token_seq=batch.token_seq, token_pos=batch.token_pos, tile_tok0=batch.tile_tok0, tile_rows=batch.tile_rows)
+    for bad in (dict(tile_tok0=batch.tile_tok0 + 400), dict(tile_tok0=batch.tile_tok0 - 300), dict(tile_rows=batch.tile_rows * 1000),
+                dict(tile_rows=batch.tile_rows * 0), dict(token_seq=batch.token_seq + 7), dict(token_seq=batch.token_seq - 3),
+                dict(token_pos=batch.token_pos + 10 ** 6), dict(token_pos=batch.token_pos - 10 ** 6), dict()):
+        K.attention_prefill_kv8(q, out, kp, vp, plan, **{**good, **bad}, n_heads=8, scale=0.1)
+        torch.cuda.synchronize()
+        assert int(flags[0]) == (3 if bad else 0), bad.keys()
+        flags.zero_()
+        assert (store[0] == 7.0).all() and (store[501] == 7.0).all()
+
+
 def test_infinities_and_nan_in_masked_places():
     """What a query does not see may hold anything: rows behind the newest (the Rig's tails), blocks before a window."""
     p = 400

@@ -65,6 +65,16 @@ def test_the_cache_still_holds_what_a_step_needs(case):
             assert not req.droppable(b, s, 64)
 
 
+@pytest.mark.parametrize("bad", [dict(window_kind=5), dict(window_kind=1, window_size=0), dict(window_kind=2, window_size=1 << 40), dict(keep_first=-1),
+                                 dict(scale=0.0), dict(scale=float("nan")), dict(softcap=-1.0), dict(softcap=float("nan")), dict(sink=torch.zeros(3)),
+                                 dict(sink=torch.zeros(4, dtype=torch.float64))])
+def test_options_refused(bad):
+    good = dict(scale=1.0, window_kind=0, window_size=0, keep_first=0, sink=None, softcap=0.0)
+    K._attention_options("test", 4, *good.values())
+    with pytest.raises(K.KernelError):
+        K._attention_options("test", 4, *{**good, **bad}.values())
+
+
 def test_plan_refusals():
     good = dict(starts=[0], n_new=[1], slots=[0], device="cpu")
     Kv8Plan(**good)
