@@ -1091,11 +1091,16 @@ _INT, _LONG, _FLOAT, _PTR = c_int, c_long, c_float, c_void_p
 _KV8_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 
 
-@functools.lru_cache(maxsize=None)
+_functions = {}
+
+
 def _declared(name: str, types: str):
     """The library's function `name` with its arguments declared: p a pointer (int or None), i int, l long, f float."""
-    fn = getattr(load(), name)
-    fn.argtypes = [{"p": _PTR, "i": _INT, "l": _LONG, "f": _FLOAT}[t] for t in types]
+    fn = _functions.get(name)
+    if fn is None:
+        fn = getattr(load(), name)
+        fn.argtypes = [{"p": _PTR, "i": _INT, "l": _LONG, "f": _FLOAT}[t] for t in types]
+        _functions[name] = fn
     return fn
 
 
@@ -1119,43 +1124,47 @@ def _here(what, *ts):
 
 
 def _kv8(cache, what, n_heads=None):
-    """(format, kv heads, head size, the tensors' addresses) of a Kv8Cache after its checks; `n_heads`: the query heads that read it."""
-    k, v, k_scale, v_scale, k_tail, v_tail = cache
-    shape, fmt = k.shape, _KV8_CODES.get(k.dtype)
+    """(format, kv heads, head size, slots, the tensors' addresses) of a Kv8Cache after its checks; `n_heads`: the query heads
+    that read it."""
+    k, v, ks, vs, kt, vt = cache
+    shape, tail, f32, bf16 = k.shape, kt.shape, torch.float32, torch.bfloat16
+    fmt = _KV8_CODES.get(k.dtype)
     if fmt is None or v.dtype is not k.dtype or len(shape) != 4 or v.shape != shape:
         raise KernelError(f"{what}: codes are int8 or float8_e4m3fn [pages, kv heads, 64, head size], keys and values alike, not "
                           f"{tuple(shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
     pages, nkv, block, d = shape
-    if block != 64 or d not in (64, 128) or pages < 1 or nkv < 1:
+    if block != 64 or (d != 128 and d != 64) or pages < 1 or nkv < 1:
         raise KernelError(f"{what}: pages of 64 positions and heads of 64 or 128 elements, not {tuple(shape)}")
-    f32, bf16 = torch.float32, torch.bfloat16
-    if k_scale.dtype is not f32 or v_scale.dtype is not f32 or k_scale.shape != (pages, nkv) or v_scale.shape != (pages, nkv):
-        raise KernelError(f"{what}: scales are float32 [{pages}, {nkv}], not {tuple(k_scale.shape)} {k_scale.dtype} and {tuple(v_scale.shape)} "
-                          f"{v_scale.dtype}")
-    tail = k_tail.shape
-    if k_tail.dtype is not bf16 or v_tail.dtype is not bf16 or v_tail.shape != tail or len(tail) != 4 or tail[1:] != (nkv, 64, d):
-        raise KernelError(f"{what}: tails are bfloat16 [slots, {nkv}, 64, {d}], not {tuple(tail)} {k_tail.dtype} and {tuple(v_tail.shape)} "
-                          f"{v_tail.dtype}")
-    at = [t.data_ptr() for t in cache]
-    if (at[0] | at[1] | at[2] | at[3] | at[4] | at[5]) % 16 or not (
-            k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous() and k_tail.is_contiguous()
-            and v_tail.is_contiguous()):
+    rows = (pages, nkv)
+    if ks.dtype is not f32 or vs.dtype is not f32 or ks.shape != rows or vs.shape != rows:
+        raise KernelError(f"{what}: scales are float32 [{pages}, {nkv}], not {tuple(ks.shape)} {ks.dtype} and {tuple(vs.shape)} {vs.dtype}")
+    if kt.dtype is not bf16 or vt.dtype is not bf16 or vt.shape != tail or len(tail) != 4 or tail[1] != nkv or tail[2] != 64 or tail[3] != d:
+        raise KernelError(f"{what}: tails are bfloat16 [slots, {nkv}, 64, {d}], not {tuple(tail)} {kt.dtype} and {tuple(vt.shape)} {vt.dtype}")
+    at = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), kt.data_ptr(), vt.data_ptr()
+    if (at[0] | at[1] | at[2] | at[3] | at[4] | at[5]) & 15 or not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous()
+                                                                  and vs.is_contiguous() and kt.is_contiguous() and vt.is_contiguous()):
         raise KernelError(f"{what}: the cache's tensors are contiguous and start on 16 bytes")
     if n_heads is not None and (n_heads < 1 or n_heads % nkv or n_heads // nkv > 16):
         raise KernelError(f"{what}: {n_heads} query heads over {nkv} key/value heads (groups of 1 to 16)")
-    return fmt, nkv, d, at
+    return fmt, nkv, d, tail[0], at
 
 
 def _i32(what, n, *ts):
+    """The addresses of index tensors: contiguous int32, of n elements unless that is None."""
     for t in ts:
         if t.dtype is not torch.int32 or not t.is_contiguous() or (n is not None and t.numel() != n):
             raise KernelError(f"{what}: indices are contiguous int32" + ("" if n is None else f" [{n}]") + f", not {t.dtype} {tuple(t.shape)}")
+    return [t.data_ptr() for t in ts]
 
 
-def _bf16_rows(what, shape, *ts):
-    for t in ts:
-        if t.dtype is not torch.bfloat16 or t.shape != shape or not t.is_contiguous() or t.data_ptr() % 16:
-            raise KernelError(f"{what}: expected contiguous bfloat16 {tuple(shape)} from 16 bytes on, not {t.dtype} {tuple(t.shape)}")
+def _bf16_rows(what, shape, a, b):
+    """The addresses of two contiguous bfloat16 tensors of `shape` that start on 16 bytes."""
+    bf16, pa, pb = torch.bfloat16, a.data_ptr(), b.data_ptr()
+    if (a.dtype is not bf16 or b.dtype is not bf16 or a.shape != shape or b.shape != shape or not a.is_contiguous() or not b.is_contiguous()
+            or (pa | pb) & 15):
+        raise KernelError(f"{what}: expected contiguous bfloat16 {tuple(shape)} from 16 bytes on, not {a.dtype} {tuple(a.shape)} and {b.dtype} "
+                          f"{tuple(b.shape)}")
+    return pa, pb
 
 
 def _attention_options(what, n_heads, scale, window_kind, window_size, keep_first, sink, softcap):
@@ -1197,30 +1206,29 @@ def attention_decode_kv8(q, out, cache, page_table, token_seq, token_pos, seq_sl
     end: no kernel of this library may be writing them (copies and other kernels have ended by then).  An index outside
     of the cache sets the error word (`device_error_flags`) and gives zeros; nothing is read or written for it."""
     what = "attention_decode_kv8"
-    fmt, nkv, d, at = _kv8(cache, what, n_heads)
-    T, k_tail = q.shape[0], cache.k_tail
-    here = _here(what, q, out, *cache, page_table, token_seq, token_pos, seq_slot)
+    fmt, nkv, d, slots, at = _kv8(cache, what, n_heads)
+    T, table = q.shape[0], page_table.shape
+    here = _here(what, q, out, page_table, token_seq, token_pos, seq_slot, *cache)
+    sink_at = None
     if sink is not None:
-        _here(what, sink)
-    _bf16_rows(what, (T, n_heads * d), q, out)
-    _i32(what, T, token_seq, token_pos)
-    _i32(what, None, seq_slot, page_table)
-    table = page_table.shape
-    if len(table) != 2 or T > 65535 or table[0] < k_tail.shape[0]:
-        raise KernelError(f"{what}: a page table [slots, blocks] for {k_tail.shape[0]} slots and up to 65535 tokens, not {tuple(table)} and {T}")
+        _here(what, q, sink)
+        sink_at = sink.data_ptr()
+    q_at, out_at = _bf16_rows(what, (T, n_heads * d), q, out)
+    seq_at, pos_at = _i32(what, T, token_seq, token_pos)
+    slot_at, table_at = _i32(what, None, seq_slot, page_table)
+    if len(table) != 2 or T > 65535 or table[0] < slots:
+        raise KernelError(f"{what}: a page table [slots, blocks] for {slots} slots and up to 65535 tokens, not {tuple(table)} and {T}")
     _attention_options(what, n_heads, scale, window_kind, window_size, keep_first, sink, softcap)
     if T == 0:
         return
     longest = min(int(max_context), table[1] * 64)
-    if window_kind != WINDOW_FULL:
+    if window_kind:
         longest = min(longest, window_size + 64 + -(-keep_first // 64) * 64)
     splits, joined = _kv8_splits(here, T * nkv, -(-max(longest, 1) // 64))
     scratch = torch.empty(T * n_heads * splits * (d + 2), dtype=torch.float32, device=q.device) if joined else None
-    _run(_declared("cpi_attention_decode_kv8", "ppppppippipipppiiiiiiiiiffpippp"),
-         q.data_ptr(), out.data_ptr(), at[0], at[1], at[2], at[3], cache.k.shape[0], at[4], at[5], k_tail.shape[0], page_table.data_ptr(), table[1],
-         token_seq.data_ptr(), token_pos.data_ptr(), seq_slot.data_ptr(), seq_slot.numel(), T, n_heads, nkv, d, fmt, window_kind, int(window_size),
-         int(keep_first), scale, softcap or 0.0, None if sink is None else sink.data_ptr(), splits, None if scratch is None else scratch.data_ptr(),
-         _flag(here), _raw_stream(here))
+    _run(_declared("cpi_attention_decode_kv8", "ppppppippipipppiiiiiiiiiffpippp"), q_at, out_at, at[0], at[1], at[2], at[3], cache[0].shape[0],
+         at[4], at[5], slots, table_at, table[1], seq_at, pos_at, slot_at, seq_slot.numel(), T, n_heads, nkv, d, fmt, window_kind, window_size,
+         keep_first, scale, softcap or 0.0, sink_at, splits, scratch.data_ptr() if joined else None, _flag(here), _raw_stream(here))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1239,16 +1247,15 @@ def kv8_stage(cache, page_table, plan, k_pages, v_pages):
     behind them, writes the blocks that are complete now to the cache and each sequence's open block to its tail, and puts
     the numbers that earlier blocks stand for into the earlier pages."""
     what = "kv8_stage"
-    fmt, nkv, d, at = _kv8(cache, what)
-    slots, table = cache.k_tail.shape[0], page_table.shape
-    here = _here(what, *cache, page_table, plan.jobs, k_pages, v_pages)
-    _bf16_rows(what, (plan.n_pages, nkv, 64, d), k_pages, v_pages)
-    _i32(what, None, page_table)
+    fmt, nkv, d, slots, at = _kv8(cache, what)
+    table, jobs = page_table.shape, plan.jobs
+    here = _here(what, k_pages, v_pages, page_table, jobs, *cache)
+    k_at, v_at = _bf16_rows(what, (plan.n_pages, nkv, 64, d), k_pages, v_pages)
+    table_at, = _i32(what, None, page_table)
     if len(table) != 2 or table[0] < slots or table[1] < plan.width:
         raise KernelError(f"{what}: a page table {tuple(table)} for {slots} slots and blocks up to {plan.width}")
-    _run(_declared("cpi_kv8_stage", "pipiippppippppiiiipp"), plan.jobs.data_ptr(), plan.n_jobs, page_table.data_ptr(), table[1], slots, at[0], at[1],
-         at[2], at[3], cache.k.shape[0], at[4], at[5], k_pages.data_ptr(), v_pages.data_ptr(), plan.n_pages, nkv, d, fmt, _flag(here),
-         _raw_stream(here))
+    _run(_declared("cpi_kv8_stage", "pipiippppippppiiiipp"), jobs.data_ptr(), plan.n_jobs, table_at, table[1], slots, at[0], at[1], at[2], at[3],
+         cache[0].shape[0], at[4], at[5], k_at, v_at, plan.n_pages, nkv, d, fmt, _flag(here), _raw_stream(here))
 
 
 def attention_prefill_kv8(q, out, k_pages, v_pages, plan, token_seq, token_pos, tile_tok0, tile_rows, *, n_heads, scale,
@@ -1264,24 +1271,25 @@ def attention_prefill_kv8(q, out, k_pages, v_pages, plan, token_seq, token_pos, 
     if n_heads < 1 or nkv < 1 or n_heads % nkv:
         raise KernelError(f"{what}: {n_heads} query heads over {nkv} key/value heads")
     here = _here(what, q, out, k_pages, v_pages, plan.jobs, token_seq, token_pos, tile_tok0, tile_rows)
+    sink_at = None
     if sink is not None:
-        _here(what, sink)
-    _bf16_rows(what, (plan.n_tokens, n_heads * d), q, out)
-    _bf16_rows(what, (plan.n_pages, nkv, 64, d), k_pages, v_pages)
-    _i32(what, plan.n_tokens, token_seq, token_pos)
+        _here(what, q, sink)
+        sink_at = sink.data_ptr()
+    q_at, out_at = _bf16_rows(what, (plan.n_tokens, n_heads * d), q, out)
+    k_at, v_at = _bf16_rows(what, (plan.n_pages, nkv, 64, d), k_pages, v_pages)
+    seq_at, pos_at = _i32(what, plan.n_tokens, token_seq, token_pos)
     tiles = tile_tok0.numel()
-    _i32(what, tiles, tile_tok0, tile_rows)
+    tok0_at, rows_at = _i32(what, tiles, tile_tok0, tile_rows)
     _attention_options(what, n_heads, scale, window_kind, window_size, keep_first, sink, softcap)
     window = (window_kind, window_size if window_kind else 0, keep_first if window_kind == WINDOW_SLIDING else 0)
     if window != (WINDOW_KINDS[plan.window[0]], *plan.window[1:]):
         raise KernelError(f"{what}: window kind {window_kind} of {window_size}, {keep_first} kept: the plan was made for {plan.window}")
     splits = _kv8_prefill_splits(here, tiles * n_heads, plan.most_tiles)
     scratch = None if splits == 1 else torch.empty(plan.n_tokens * n_heads * splits * (d + 2), dtype=torch.float32, device=q.device)
-    _run(_declared("cpi_attention_prefill_kv8", "pppplppiippppiiiiiiiiffpippp"), q.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-         plan.n_pages, plan.earlier_table.data_ptr(), plan.exact_table.data_ptr(), plan.n_seqs, plan.width, token_seq.data_ptr(), token_pos.data_ptr(),
-         tile_tok0.data_ptr(), tile_rows.data_ptr(), tiles, plan.n_tokens, n_heads, nkv, d, window_kind, int(window_size), int(keep_first), scale,
-         softcap or 0.0, None if sink is None else sink.data_ptr(), splits, None if scratch is None else scratch.data_ptr(), _flag(here),
-         _raw_stream(here))
+    _run(_declared("cpi_attention_prefill_kv8", "pppplppiippppiiiiiiiiffpippp"), q_at, out_at, k_at, v_at, plan.n_pages,
+         plan.earlier_table.data_ptr(), plan.exact_table.data_ptr(), plan.n_seqs, plan.width, seq_at, pos_at, tok0_at, rows_at, tiles,
+         plan.n_tokens, n_heads, nkv, d, window_kind, window_size, keep_first, scale, softcap or 0.0, sink_at, splits,
+         None if scratch is None else scratch.data_ptr(), _flag(here), _raw_stream(here))
 
 
 @functools.lru_cache(maxsize=4096)
