@@ -29,6 +29,7 @@
 // Rows of masked positions are zeros before they are multiplied: what an earlier sequence left cannot reach a result.
 // Waits are bounded as in attention_decode.cu.
 #include "kv8.cuh"
+#include "packed.cuh"
 #include <cuda.h>
 
 namespace cpi {
@@ -810,3 +811,4 @@ extern "C" int cpi_attention_decode_kv8(const void* q, void* out, void* k, void*
   return fmt ? CPI_DEC8(64, 1) : CPI_DEC8(64, 0);
 #undef CPI_DEC8
 }
+CPI_PACKED(cpi_attention_decode_kv8)

@@ -28,14 +28,6 @@
 // and 4,096 tokens 324 (530 TFLOP/s).  The cap compiled apart, a row's mask as one word per 32 columns and a small loop for the
 // first tile's maximum: 8.4, 138 and 226 us (760; 961 at 16,384 tokens).
 //
-// BLOCKED: attention over the cache in 8 bits (kv8.cuh).  A query sees its own block of 64 positions as projected and earlier
-// blocks as the numbers they are held as; both stand in bfloat16 pages of the step's own, named by two tables.  The axis of key
-// tiles then begins with the exact tiles of query tile A, goes on with the earlier blocks' and ends with the exact tiles of B: A
-// meets a prefix of it and B a suffix, as without BLOCKED.  A row's mask is that of the window cut at the start of its block,
-// from one side or the other.  Pages that a tile does not have are asked for beyond the tensor's end and arrive as zeros, rows
-// behind the newest position are zero already: nothing is overwritten in shared memory.  Per query tile that is one or two key
-// tiles more than without (they hold the own blocks twice).
-//
 // Every mbarrier wait is bounded; when one runs out the CTA sets *error_flag and leaves.
 #include "prefill_tc.cuh"
 #include <type_traits>
@@ -57,20 +49,12 @@ struct Params {
   const float* sink;                  // [NH] float32 or null: exp(sink[h]) joins the softmax denominator (no key, no value)
   int keep_first;                     // sliding window: a sequence's first positions stay visible to every later query
   float cap_in, cap_out;              // soft cap c > 0 on the scaled scores: cap_in = scale / c, cap_out = c log2(e); else 0
-  const int* exact_table;             // BLOCKED: pages by sequence of the step and block (page_table: those of earlier blocks), -1 none
-  int n_pages, n_tokens, n_seqs;
-  int n_splits;                       // BLOCKED: blocks of threads that share a query tile's axis of key tiles
-  float* part_o; float2* part_ml;     // with several: [T, NH, splits, D] sums, [T, NH, splits] reference and row sum
 };
 
 
-// BLOCKED raises a row's reference only by 2^40: P is bfloat16 and the sums are float32, which have the same range of powers, so
-// nothing is lost by numbers up to 2^40 (sums up to 2^57, outputs finite for values up to 2^70), and a pass is hardly ever
-// repeated (keys and queries with a few large features, 3,001 tokens of 40 heads: 190 us with 2^8, 171 with 2^40).
-constexpr float kWideSlack = 40.0f;
 constexpr int kRingSlots = 5;           // key and value tiles in shared memory at a time
 
-template <int D, bool CAPPED, bool BLOCKED = false>
+template <int D, bool CAPPED>
 __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                 const __grid_constant__ CUtensorMap map_k,
                                                                 const __grid_constant__ CUtensorMap map_v, Params p) {
@@ -111,22 +95,10 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
   pdl_launch_dependents();                              // (in this order, and not before the tensor memory is ours: see common.cuh)
   const int tile = blockIdx.y, head = blockIdx.x;       // heads are the fast axis: all heads of the longest tile start first
   const int kvh = head / (p.n_heads / p.n_kv_heads);
-  int tok0 = p.tile_tok0[tile], rows = p.tile_rows[tile];
-  if (BLOCKED) {                                        // indices outside of the step: somewhere within it, and the error flag
-    const bool good = tok0 >= 0 && tok0 < p.n_tokens && rows >= 1 && rows <= kTileRows && rows <= p.n_tokens - tok0;
-    tok0 = min(max(tok0, 0), p.n_tokens - 1);
-    rows = min(max(rows, 1), min(kTileRows, p.n_tokens - tok0));
-    if (!good && tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
-  }
-  int slot = BLOCKED ? p.token_seq[tok0] : p.seq_slot[p.token_seq[tok0]];
+  const int tok0 = p.tile_tok0[tile], rows = p.tile_rows[tile];
+  const int slot = p.seq_slot[p.token_seq[tok0]];
   // the tile's rows are consecutive positions of one sequence; rows 0-127 are query tile A, the rest tile B
-  int pos_first = p.token_pos[tok0];
-  if (BLOCKED && (slot < 0 || slot >= p.n_seqs || pos_first < 0 || pos_first > p.max_blocks * PAGE - rows)) {
-    slot = 0;
-    pos_first = 0;
-    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
-  }
-  const int pos_last = pos_first + rows - 1;
+  const int pos_first = p.token_pos[tok0], pos_last = pos_first + rows - 1;
   const int rows_x[2] = {min(rows, BQ), max(rows - BQ, 0)};
   const bool has_b = rows_x[1] > 0;
   const int p0_x[2] = {pos_first, pos_first + BQ};                         // first position of A, of B
@@ -143,31 +115,10 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
   const int keep = p.window_kind == 2 ? p.keep_first : 0;
   const int n_kept = min((keep + BKV - 1) / BKV, kb_phys[0]);
   const int gap = kb_phys[0] - n_kept;
-  // BLOCKED: exact tiles of A, then earlier blocks' tiles up to the one that holds the last position before A's (B's) last
-  // row's block, then exact tiles of B
-  const int first_exact[2] = {p0_x[0] / BKV, p0_x[1] / BKV};
-  const int n_exact[2] = {BLOCKED ? p1_x[0] / BKV - first_exact[0] + 1 : 0, BLOCKED && has_b ? p1_x[1] / BKV - first_exact[1] + 1 : 0};
-  auto tiles_to = [&](int x) { return BLOCKED ? max((p1_x[x] / PAGE * PAGE + BKV - 1) / BKV - gap, 0) : p1_x[x] / BKV + 1 - gap; };
-  const int n_earlier = tiles_to(has_b ? 1 : 0);
-  int kb_x[2] = {0, n_exact[0] + (has_b && keep == 0 ? kb_phys[1] - gap : 0)};
-  int ke_x[2] = {n_exact[0] + tiles_to(0), has_b ? n_exact[0] + n_earlier + n_exact[1] : 0};
-  int kt0 = 0, kt1 = has_b ? ke_x[1] : ke_x[0];                           // the union: every tile in it is met by A or B
-  if (BLOCKED && p.n_splits > 1) {                                        // this block's share of the union
-    const int per = (kt1 + p.n_splits - 1) / p.n_splits;
-    kt0 = min(kt1, (int)blockIdx.z * per);
-    kt1 = min(kt1, kt0 + per);
-#pragma unroll
-    for (int x = 0; x < 2; ++x) { kb_x[x] = min(max(kb_x[x], kt0), kt1); ke_x[x] = max(min(ke_x[x], kt1), kb_x[x]); }
-  }
-  auto is_exact = [&](int kt) { return BLOCKED && (kt < n_exact[0] || kt >= n_exact[0] + n_earlier); };
-  auto key_tile = [&](int kt) {
-    if (BLOCKED) {
-      if (kt < n_exact[0]) return first_exact[0] + kt;
-      kt -= n_exact[0];
-      if (kt >= n_earlier) return first_exact[1] + kt - n_earlier;
-    }
-    return kt < n_kept ? kt : kt + gap;
-  };
+  const int kb_x[2] = {0, has_b && keep == 0 ? kb_phys[1] - gap : 0};
+  const int ke_x[2] = {p1_x[0] / BKV + 1 - gap, has_b ? p1_x[1] / BKV + 1 - gap : 0};
+  const int kt0 = 0, kt1 = has_b ? ke_x[1] : ke_x[0];                     // the union: every tile in it is met by A or B
+  auto key_tile = [&](int kt) { return kt < n_kept ? kt : kt + gap; };
   const uint32_t tmem_s = tmem_base_s, tmem_o = tmem_base_s + 256;        // + 128 for tile B, both
   volatile int* abort_flag = &abort_s;
   bool ok = true;
@@ -184,22 +135,14 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
       int n = 0;                                         // item of the ring: 2 (kt - kt0) for keys, + 1 for values
       for (int kt = kt0; kt < kt1 && ok; ++kt) {
         const int blk0 = key_tile(kt) * (BKV / PAGE);
-        const int n_pages = BLOCKED ? BKV / PAGE : min(BKV / PAGE, last_block - blk0 + 1);
-        const int* pages = BLOCKED && is_exact(kt) ? p.exact_table + (size_t)slot * p.max_blocks : table;
+        const int n_pages = min(BKV / PAGE, last_block - blk0 + 1);
         const uint32_t bytes = (uint32_t)n_pages * HALVES * (PAGE * 128);
         for (int which = 0; which < 2; ++which, ++n) {
           const int s = n % NSLOT;
           if (n >= NSLOT && !mbar_wait(&kv_empty[s], ((n / NSLOT) - 1) & 1, abort_flag)) { ok = false; break; }
           mbar_expect_tx(&kv_full[s], bytes);
           for (int pg = 0; pg < n_pages; ++pg) {
-            int page = 0;
-            if (BLOCKED) {                               // a page that the step does not have: beyond the tensor, zeros
-              page = blk0 + pg < p.max_blocks ? pages[blk0 + pg] : -1;
-              if (page < 0 || page >= p.n_pages) page = p.n_pages;
-            } else {
-              page = table[blk0 + pg];
-            }
-            const int row = (page * p.n_kv_heads + kvh) * PAGE;
+            const int row = (table[blk0 + pg] * p.n_kv_heads + kvh) * PAGE;
             for (int h = 0; h < HALVES; ++h)
               tma_load_2d(ring + s * KV_BYTES + h * HALF_BYTES + pg * (PAGE * 128), which ? &map_v : &map_k,
                           &kv_full[s], h * 64, row);
@@ -274,9 +217,8 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
       return true;
     };
     ok = __all_sync(0xffffffffu, mbar_wait(&q_full, 0, abort_flag));
-    // (a share of the union may have nothing for A, or nothing for B)
-    const int kb_b = has_b && (!BLOCKED || kb_x[1] < ke_x[1]) ? kb_x[1] : 0x7fffffff, ke_a = ke_x[0];
-    if (!BLOCKED || ke_a > kt0) ok = ok && issue_qk(0, kb_b != kt0);
+    const int kb_b = has_b ? kb_x[1] : 0x7fffffff, ke_a = ke_x[0];
+    ok = ok && issue_qk(0, kb_b != kt0);
     if (ok && kb_b == kt0) ok = issue_qk(1, true);
     for (int kt = kt0; kt < kt1 && ok; ++kt) {
       // which query tiles meet key tile kt, and kt + 1 (B's range ends with the union's, A's begins with it)
@@ -310,9 +252,7 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
     const float sc = CAPPED ? p.cap_out : p.scale_log2, cap_in = p.cap_in;
     // the union's last key tile holds positions beyond the newest one: their value rows are zeroed by the group
     // whose P V on that tile is issued first (A if it meets the tile, otherwise B)
-    const int edge = BLOCKED && live ? qp / PAGE * PAGE : 0;        // the row's own block begins here
-    const int edge_first = p0_x[x] / PAGE * PAGE;
-    const bool zero_duty = BLOCKED ? false : x == 0 ? (kt1 - 1 >= kb_x[0] && kt1 - 1 < ke_x[0]) : !(kt1 - 1 >= kb_x[0] && kt1 - 1 < ke_x[0]);
+    const bool zero_duty = x == 0 ? (kt1 - 1 >= kb_x[0] && kt1 - 1 < ke_x[0]) : !(kt1 - 1 >= kb_x[0] && kt1 - 1 < ke_x[0]);
     int j = 0;
     bool okl = rows_x[x] > 0;
     for (int kt = kb_x[x]; kt < ke_x[x] && okl; ++kt, ++j) {
@@ -336,106 +276,7 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
       if (!okl) break;
       fence_after_sync();
       // a tile that lies wholly inside every row's window needs no position tests
-      const bool exact = is_exact(kt);
-      const bool no_mask = (BLOCKED ? !exact && key0 + BKV <= edge_first : key0 + BKV - 1 <= p0_x[x]) &&
-                           (key0 >= lo_last || key0 + BKV - 1 < keep);
-      auto sees = [&](int first) {
-        uint32_t in = visible(qp, lo, keep, first);
-        if (BLOCKED) {
-          const int n = edge - first;
-          const uint32_t before = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-          in &= exact ? ~before : before;
-        }
-        return in;
-      };
-      if constexpr (BLOCKED) {
-        // Small code: a block of threads meets most of it cold, and with masks on several tiles, exact and earlier ones, the
-        // pass below, four times over, is more than an instruction cache holds.  Tiles without a mask take one pass of their
-        // own against the reference they have; all others two small loops, the maximum and then the exponentials, whose
-        // P goes over columns of S that have been read.  Columns that no row of the warp sees are passed over.
-        bool stored = false;
-        auto raised = [&](float mx) {                      // the reference after a row maximum mx; O follows
-          const bool grow = mx > m_ref + (m_ref < -1e29f ? 0.f : kWideSlack);
-          if (j == 0) { m_ref = fmaxf(mx, m_ref); return; }
-          if (!__any_sync(0xffffffffu, grow)) return;
-          const float m_new = grow ? mx : m_ref, f = exp2f(m_ref - m_new);
-#pragma unroll 1
-          for (int c = 0; c < D; c += 32) {                // (every P V issued so far has landed, see below)
-            float v[32];
-            tmem_ld32(o_row + c, v);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] *= f;
-            tmem_st32(o_row + c, v);
-          }
-          l_run *= f;
-          m_ref = m_new;
-        };
-        if (!CAPPED && no_mask && j > 0) {
-          uint32_t w[BKV / 32][16], raw[2][32];
-          const float nref = -m_ref;
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, ls4[4] = {0.f, 0.f, 0.f, 0.f};
-          tmem_ld32_issue(s_row, raw[0]);
-          tmem_ld32_issue(s_row + 32, raw[1]);
-          tmem_wait_ld();
-#pragma unroll
-          for (int cc = 0; cc < BKV / 32; ++cc) {
-            float v[32];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float sv = __uint_as_float(raw[cc & 1][e]);
-              mx4[e & 3] = fmaxf(mx4[e & 3], sv);
-              v[e] = exp2_fast(fmaf(sv, sc, nref));
-            }
-            if (cc + 2 < BKV / 32) tmem_ld32_issue(s_row + (cc + 2) * 32, raw[cc & 1]);     // this buffer is consumed
-#pragma unroll
-            for (int e = 0; e < 32; ++e) ls4[e & 3] += v[e];
-#pragma unroll
-            for (int g = 0; g < 16; ++g) w[cc][g] = pack_bf16(v[2 * g], v[2 * g + 1]);
-            if (cc == 1) tmem_wait_ld();
-          }
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
-          stored = !__any_sync(0xffffffffu, mx > m_ref + (m_ref < -1e29f ? 0.f : kWideSlack));
-          if (stored) {
-#pragma unroll
-            for (int cc = 0; cc < BKV / 32; ++cc) tmem_st16_nowait(s_row + cc * 16, w[cc]);
-            l_run += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
-          }
-        }
-        if (!stored) {
-          float mx = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < BKV; c += 32) {
-            const uint32_t in = no_mask ? 0xffffffffu : sees(key0 + c);
-            if (!__any_sync(0xffffffffu, in != 0)) continue;
-            float v[32], mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            tmem_ld32(s_row + c, v);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], (in >> e) & 1u ? v[e] : -INFINITY);
-            mx = fmaxf(mx, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
-          }
-          raised(CAPPED && mx > -INFINITY ? tanh_fast(mx * cap_in) * sc : mx * sc);
-          const float nref = -m_ref;
-#pragma unroll 1
-          for (int c = 0; c < BKV; c += 32) {
-            const uint32_t in = no_mask ? 0xffffffffu : sees(key0 + c);
-            uint32_t w[16] = {};
-            if (__any_sync(0xffffffffu, in != 0)) {
-              float v[32], ls4[4] = {0.f, 0.f, 0.f, 0.f};
-              tmem_ld32(s_row + c, v);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                if (CAPPED) v[e] = tanh_fast(v[e] * cap_in);
-                v[e] = (in >> e) & 1u ? exp2_fast(fmaf(v[e], sc, nref)) : 0.f;
-                ls4[e & 3] += v[e];
-              }
-#pragma unroll
-              for (int g = 0; g < 16; ++g) w[g] = pack_bf16(v[2 * g], v[2 * g + 1]);
-              l_run += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
-            }
-            tmem_st16_nowait(s_row + (c >> 1), w);
-          }
-        }
-      } else {
+      const bool no_mask = key0 + BKV - 1 <= p0_x[x] && (key0 >= lo_last || key0 + BKV - 1 < keep);
       // One pass over the row's 128 columns of S, 32 at a time with the next chunk's load in flight: the
       // maximum, P = 2^(s c - ref) as packed bf16, and the sum.  P is kept in registers until the pass is
       // known to stand, because it goes over the S it came from.
@@ -449,7 +290,7 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
         for (int c = 0; c < BKV; c += 32) {
           float v[32], mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           tmem_ld32(s_row + c, v);
-          const uint32_t in = sees(key0 + c);
+          const uint32_t in = visible(qp, lo, keep, key0 + c);
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             if (CAPPED) v[e] = tanh_fast(v[e] * cap_in);
@@ -478,7 +319,7 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
               v[e] = exp2_fast(fmaf(sv, sc, nref));
             }
           } else {
-            const uint32_t in = sees(key0 + cc * 32);
+            const uint32_t in = visible(qp, lo, keep, key0 + cc * 32);
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               float sv = __uint_as_float(raw[cc & 1][e]);
@@ -522,7 +363,6 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
 #pragma unroll
       for (int cc = 0; cc < BKV / 32; ++cc) tmem_st16_nowait(s_row + cc * 16, w[cc]);
       l_run += ls;
-      }
       tmem_wait_st();
       fence_before_sync();
       __syncwarp();
@@ -530,27 +370,11 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
     }
     // the output: O / l once the last P V is done
     ok = okl && !abort_s && j > 0;
-    if (BLOCKED && p.n_splits > 1 && live) {
-      // what this share adds up to: the row's sums and what they are measured against (nothing: a sum of zero)
-      p.part_ml[((size_t)(tok0 + x * BQ + row) * p.n_heads + head) * p.n_splits + blockIdx.z] = make_float2(m_ref, j > 0 ? l_run : 0.f);
-    }
     ok = __all_sync(0xffffffffu, ok && mbar_wait(&o_done[x], 0, abort_flag));
     fence_after_sync();
     if (ok) {
       // a sink adds 2^(sink log2 e - reference) to the row's sum and nothing to O; the exponent is capped so that a
       // sink far above every score gives a huge finite sum
-      if (BLOCKED && p.n_splits > 1) {
-        float* dst = p.part_o + (((size_t)(tok0 + x * BQ + row) * p.n_heads + head) * p.n_splits + blockIdx.z) * D;
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          float v[32];
-          tmem_ld32(o_row + c, v);
-          if (live) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(dst + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-          }
-        }
-      } else {
       if (p.sink) l_run += exp2f(fminf(p.sink[head] * 1.4426950408889634f - m_ref, 120.f));
       const float inv = 1.0f / fmaxf(l_run, 1e-20f);
       __nv_bfloat16* dst = p.out + ((size_t)(tok0 + x * BQ + row) * p.n_heads + head) * D;
@@ -567,7 +391,6 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
           }
         }
       }
-      }
     }
     fence_before_sync();
   }
@@ -578,41 +401,6 @@ __global__ void __launch_bounds__(kThreads) attention_prefill_kernel(const __gri
   fence_before_sync();
   __syncthreads();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_s), "r"(TMEM_COLS));
-}
-
-// The shares of a query tile's keys joined: out[t, h] = sum_s w_s O_s / (sum_s w_s l_s + sink), w_s = 2^(m_s - max m).  A warp per
-// (token, head), four features or two per lane.
-template <int D>
-__global__ void __launch_bounds__(256) attention_prefill_combine(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
-                                                                 __nv_bfloat16* __restrict__ out, long rows, int n_splits,
-                                                                 const float* __restrict__ sink, int n_heads) {
-  constexpr int PER = D / 32;
-  const int lane = threadIdx.x & 31;
-  const long th = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  pdl_wait();
-  pdl_launch_dependents();
-  if (th >= rows) return;
-  const float2 ml = lane < n_splits ? __ldcg(part_ml + th * n_splits + lane) : make_float2(-1e30f, 0.f);
-  const float M = warp_max(ml.x);
-  const float w = exp2f(ml.x - M), l = ml.y > 0.f || ml.y != ml.y ? w * ml.y : 0.f;
-  float L = warp_sum(l), acc[PER] = {};
-  for (int s = 0; s < n_splits; ++s) {
-    const float ws = __shfl_sync(0xffffffffu, w, s), ls = __shfl_sync(0xffffffffu, ml.y, s);
-    if (ls == 0.f) continue;                             // (this share held nothing for the row, or was not written)
-    const float* src = part_o + (th * n_splits + s) * D + lane * PER;
-    if (PER == 4) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-      acc[0] += ws * v.x; acc[1] += ws * v.y; acc[PER - 2] += ws * v.z; acc[PER - 1] += ws * v.w;
-    } else {
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-      acc[0] += ws * v.x; acc[1] += ws * v.y;
-    }
-  }
-  if (sink) L += exp2f(fminf(sink[th % n_heads] * 1.4426950408889634f - M, 120.f));
-  const float inv = 1.0f / fmaxf(L, 1e-20f);
-  uint32_t* dst = reinterpret_cast<uint32_t*>(out + th * D + lane * PER);
-#pragma unroll
-  for (int i = 0; i < PER / 2; ++i) dst[i] = pack_bf16(acc[2 * i] * inv, acc[2 * i + 1] * inv);
 }
 
 }  // namespace pre
@@ -651,7 +439,7 @@ extern "C" int cpi_attention_prefill(const void* q, void* out, const void* k_cac
   pre::Params p{(__nv_bfloat16*)out, page_table, max_blocks, token_pos, token_seq, seq_slot, tile_tok0, tile_rows,
                 n_heads, n_kv_heads, window_kind, window_size, scale * 1.4426950408889634f, error_flag, sink,
                 keep_first > 0 ? keep_first : 0, softcap > 0.f ? scale / softcap : 0.f,
-                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, nullptr, 0, 0, 0, 1, nullptr, nullptr};
+                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f};
   dim3 grid(n_heads, n_tiles);
   const int halves = head_dim / 64;
   const int smem = halves * 128 * 128 * (2 + pre::kRingSlots);     // Q of both tiles, the ring of K and V tiles
@@ -666,58 +454,4 @@ extern "C" int cpi_attention_prefill(const void* q, void* out, const void* k_cac
   };
   if (head_dim == 128) launch_dim(std::integral_constant<int, 128>{}); else launch_dim(std::integral_constant<int, 64>{});
   return check_launch("attention_prefill");
-}
-
-// The same over the pages of a step on the cache in 8 bits: k_pages, v_pages [n_pages, NKV, 64, D] bfloat16, named per sequence of the
-// step and block by earlier_table and exact_table [sequences, width] (-1: none).  `n_splits` > 1: that many blocks of threads share a query tile's
-// keys, through `scratch` (n_tokens * n_heads * n_splits * (head_dim + 2) floats).
-extern "C" int cpi_attention_prefill_kv8(const void* q, void* out, const void* k_pages, const void* v_pages, long n_pages,
-                                         const int* earlier_table, const int* exact_table, int n_seqs, int width, const int* token_seq,
-                                         const int* token_pos, const int* tile_tok0, const int* tile_rows, int n_tiles, int n_tokens,
-                                         int n_heads, int n_kv_heads, int head_dim, int window_kind, int window_size, int keep_first,
-                                         float scale, float softcap, const float* sink, int n_splits, float* scratch, int* error_flag,
-                                         cudaStream_t stream) {
-  if (n_tiles == 0 || n_tokens == 0) return 0;
-  const long rows = (long)n_tokens * n_heads;
-  CPI_REQUIRE(n_splits >= 1 && n_splits <= 32 && (n_splits == 1 || scratch), "attention_prefill_kv8: %d shares (up to 32, with scratch)", n_splits);
-  CPI_REQUIRE(cpi_attention_prefill_supported(n_heads, n_kv_heads, head_dim, pre::PAGE),
-              "attention_prefill_kv8: unsupported shape (heads %d/%d, head size %d)", n_heads, n_kv_heads, head_dim);
-  CPI_REQUIRE(window_kind == 0 || window_size > 0, "attention_prefill_kv8: window kind %d needs a size > 0", window_kind);
-  CPI_REQUIRE(n_tiles <= 65535, "attention_prefill_kv8: too many query tiles in one launch (%d)", n_tiles);
-  const uint64_t kv_rows = (uint64_t)n_pages * n_kv_heads * pre::PAGE;
-  CPI_REQUIRE(n_pages > 0 && kv_rows + (uint64_t)n_kv_heads * pre::PAGE < (1ull << 31), "attention_prefill_kv8: %ld pages of %d heads", n_pages, n_kv_heads);
-  CUtensorMap mq, mk, mv;
-  const uint64_t q_width = (uint64_t)n_heads * head_dim;
-  if (tc::get_map_2d_bf16(q, q_width, (uint64_t)n_tokens, q_width * 2, 64, pre::BQ, &mq)) return 1;
-  if (tc::get_map_2d_bf16(k_pages, (uint64_t)head_dim, kv_rows, (uint64_t)head_dim * 2, 64, pre::PAGE, &mk)) return 1;
-  if (tc::get_map_2d_bf16(v_pages, (uint64_t)head_dim, kv_rows, (uint64_t)head_dim * 2, 64, pre::PAGE, &mv)) return 1;
-  pre::Params p{(__nv_bfloat16*)out, earlier_table, width, token_pos, token_seq, nullptr, tile_tok0, tile_rows,
-                n_heads, n_kv_heads, window_kind, window_size, scale * 1.4426950408889634f, error_flag, sink,
-                keep_first > 0 ? keep_first : 0, softcap > 0.f ? scale / softcap : 0.f,
-                softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, exact_table, (int)n_pages, n_tokens, n_seqs, n_splits, scratch,
-                scratch ? reinterpret_cast<float2*>(scratch + rows * n_splits * head_dim) : nullptr};
-  dim3 grid(n_heads, n_tiles, n_splits);
-  // One block of threads to an SM: each takes all of the tensor memory.  Two heads' worth of 64 would fit an SM's shared memory, and
-  // a second block that is put there, while the kernel before still fills the other SMs, waits for the first to end (four windowed
-  // prompts, 144 blocks: 80 us instead of 47).
-  const int smem = head_dim == 64 ? 120 * 1024 : head_dim / 64 * 128 * 128 * (2 + pre::kRingSlots);
-  auto launch = [&](auto dim, auto capped) {
-    auto* kernel = pre::attention_prefill_kernel<dim.value, capped.value, true>;
-    static bool set[64] = {};                              // per device
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !set[dev]) {
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      if (dev >= 0 && dev < 64) set[dev] = true;
-    }
-    cpi::launch_pdl(kernel, grid, pre::kThreads, smem, stream, mq, mk, mv, p);
-  };
-  auto launch_dim = [&](auto dim) {
-    if (p.cap_out > 0.f) launch(dim, std::true_type{}); else launch(dim, std::false_type{});
-  };
-  if (head_dim == 128) launch_dim(std::integral_constant<int, 128>{}); else launch_dim(std::integral_constant<int, 64>{});
-  if (check_launch("attention_prefill_kv8")) return 2;
-  if (n_splits == 1) return 0;
-  auto* combine = head_dim == 128 ? pre::attention_prefill_combine<128> : pre::attention_prefill_combine<64>;
-  cpi::launch_pdl(combine, dim3((unsigned)((rows + 7) / 8)), 256, 0, stream, p.part_o, p.part_ml, p.out, rows, n_splits, sink, n_heads);
-  return check_launch("attention_prefill_combine");
 }

@@ -1,0 +1,538 @@
+// Prefill attention over the cache in 8 bits (kv8.cuh) on tcgen05: two tiles of 128 queries of one head against the pages of a step.
+//
+// A query sees its own block of 64 positions as projected and earlier blocks as the numbers they are held as; both stand in
+// bfloat16 pages of the step's own, named by two tables (kv8_stage has made them).  A block of threads takes up to 256 consecutive
+// tokens of one sequence and one query head, query tile A (the first 128 rows) and B (the rest), as in attention_prefill.cu: warp 8
+// streams key/value tiles of 128 positions (two pages, TMA with the 128-byte swizzle) into a ring of five slots, K(i), V(i),
+// K(i+1), ...; one lane of warp 9 issues the MMAs, alternating between A and B, so that the tensor pipe works for one while the
+// other's softmax runs:
+//     S = Q K^T            both operands K-major from shared memory, S in tensor memory
+//     P = 2^(S*c - m)      as bfloat16 over columns of the S it came from
+//     O += P V             P as the A operand from tensor memory, V consumed MN-major from the page layout [position][dim]
+//
+// The axis of key tiles begins with the exact tiles of A (those that hold its own blocks), goes on with the earlier blocks' and ends
+// with the exact tiles of B: A meets a prefix of it and B a suffix.  A row's mask is that of the window cut at the start of its block,
+// from one side or the other.  Pages that a tile does not have are asked for beyond the tensor's end and arrive as zeros, rows behind
+// the newest position are zero already: nothing is overwritten in shared memory.  Per query tile that is one or two key tiles more
+// than over a cache in bfloat16 (they hold the own blocks twice).
+//
+// Softmax: warps 0-3 own query tile A, warps 4-7 tile B; thread r of a group owns query row r and all 128 columns of a tile.  A row's
+// reference m is raised, and O rescaled in tensor memory, only when the row maximum has outgrown it by 2^40: P is bfloat16 and the
+// sums are float32, which have the same range of powers, so nothing is lost by numbers up to 2^40 (sums up to 2^57, outputs finite
+// for values up to 2^70), and it happens in a row's first tile and hardly ever again (keys and queries with a few large features,
+// 3,001 tokens of 40 heads: 190 us with 2^8, 171 with 2^40).  Tiles without a mask take one pass against the reference they have;
+// all others two small loops, the maximum and then the exponentials, whose P goes over columns of S that have been read: a block of
+// threads meets most of this code cold, and one pass for all cases was more than an instruction cache holds.  Columns that no row of
+// the warp sees are passed over.
+//
+// Bound by the chain S -> softmax -> P V -> next S of each query tile, 4,400 cycles for two tiles of 128 x 128, where the products
+// take 2,048 and the exponentials as many.  Two threads to a row (sixteen warps) did not shorten it: with 96 registers a thread
+// either spills (238 us for 3,001 tokens of 40 heads) or reads S twice (168), against 155.
+//
+// Few query tiles over many keys share their key tiles out among blocks of threads (n_splits), joined by a second kernel.
+// Every mbarrier wait is bounded; when one runs out the block sets *error_flag and leaves.
+#include "prefill_tc.cuh"
+#include "packed.cuh"
+#include <type_traits>
+
+namespace cpi {
+namespace pre8 {
+
+using namespace pre;
+
+constexpr int PAGE = 64;
+constexpr int kRingSlots = 5;           // key and value tiles in shared memory at a time
+constexpr int kSoftmaxWarps = 8, kThreads = (kSoftmaxWarps + 2) * 32;
+constexpr float kWideSlack = 40.0f;
+
+struct Params {
+  __nv_bfloat16* out;                 // [T, NH * D]
+  const int *earlier_table, *exact_table; int width;      // pages by sequence of the step and block, -1: none
+  const int *token_pos, *token_seq;
+  const int *tile_tok0, *tile_rows;   // per query tile: first packed token, valid rows
+  int n_heads, n_kv_heads;
+  int window_kind, window_size, keep_first;
+  float scale_log2;
+  int* error_flag;
+  const float* sink;                  // [NH] float32 or null: exp(sink[h]) joins the softmax denominator (no key, no value)
+  float cap_in, cap_out;              // soft cap c > 0 on the scaled scores: cap_in = scale / c, cap_out = c log2(e); else 0
+  int n_pages, n_tokens, n_seqs;
+  int n_splits;                       // blocks of threads that share a query tile's axis of key tiles
+  float* part_o; float2* part_ml;     // with several: [T, NH, splits, D] sums, [T, NH, splits] reference and row sum
+};
+
+template <int D, bool CAPPED>
+__global__ void __launch_bounds__(kThreads, 1) attention_prefill_kv8_kernel(const __grid_constant__ CUtensorMap map_q,
+                                                                         const __grid_constant__ CUtensorMap map_k,
+                                                                         const __grid_constant__ CUtensorMap map_v, Params p) {
+  constexpr int HALVES = D / 64;                       // 64-element (128-byte) column blocks of a row
+  constexpr uint32_t HALF_BYTES = 128 * 128;           // 128 rows x 128 bytes
+  constexpr uint32_t Q_BYTES = HALVES * HALF_BYTES;    // one query tile of 128 rows
+  constexpr uint32_t KV_BYTES = HALVES * HALF_BYTES;   // one of K or V, 128 positions
+  constexpr uint32_t TMEM_COLS = 512;                  // S of tile A, S of tile B (128 columns each), O of A, O of B
+  constexpr int NSLOT = kRingSlots;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ uint64_t q_full, kv_full[NSLOT], kv_empty[NSLOT], s_full[2], p_full[2], o_done[2];
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int abort_s;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* q_s = smem_raw;                             // [2 query tiles]
+  uint8_t* ring = q_s + 2 * Q_BYTES;                   // [NSLOT]
+
+  if (tid == 0) {
+    mbar_init(&q_full, 1);
+    for (int s = 0; s < NSLOT; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_empty[s], 1); }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4); mbar_init(&o_done[s], 1);
+    }
+    abort_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  pdl_wait();
+  pdl_launch_dependents();                              // (in this order, and not before the tensor memory is ours: see common.cuh)
+  const int tile = blockIdx.y, head = blockIdx.x;       // heads are the fast axis: all heads of the longest tile start first
+  const int kvh = head / (p.n_heads / p.n_kv_heads);
+  int tok0 = p.tile_tok0[tile], rows = p.tile_rows[tile];
+  {                                                     // indices outside of the step: somewhere within it, and the error flag
+    const bool good = tok0 >= 0 && tok0 < p.n_tokens && rows >= 1 && rows <= kTileRows && rows <= p.n_tokens - tok0;
+    tok0 = min(max(tok0, 0), p.n_tokens - 1);
+    rows = min(max(rows, 1), min(kTileRows, p.n_tokens - tok0));
+    if (!good && tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+  }
+  int seq = p.token_seq[tok0];
+  // the tile's rows are consecutive positions of one sequence; rows 0-127 are query tile A, the rest tile B
+  int pos_first = p.token_pos[tok0];
+  if (seq < 0 || seq >= p.n_seqs || pos_first < 0 || pos_first > p.width * PAGE - rows) {
+    seq = 0;
+    pos_first = 0;
+    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+  }
+  const int pos_last = pos_first + rows - 1;
+  const int rows_x[2] = {min(rows, BQ), max(rows - BQ, 0)};
+  const bool has_b = rows_x[1] > 0;
+  const int p0_x[2] = {pos_first, pos_first + BQ};                         // first position of A, of B
+  const int p1_x[2] = {pos_first + rows_x[0] - 1, pos_last};               // last position of A, of B
+  // key tiles (of 128 positions) that each query tile meets; the window's low end never decreases with the position
+  const int kb_phys[2] = {window_low(p.window_kind, p.window_size, p0_x[0]) / BKV,
+                          has_b ? window_low(p.window_kind, p.window_size, p0_x[1]) / BKV : 0};
+  // Kept first positions: the key tiles that hold them and lie wholly below the window's first tile come first.
+  // The loops below count key tiles on an axis of their own, `n_kept` kept tiles (key tiles 0 .. n_kept - 1) and
+  // then the window's tiles without a gap: tile kt of the axis is key tile kt + (kt < n_kept ? 0 : gap).  With
+  // kept positions both query tiles meet every tile of the axis from its start, which always holds position 0: the
+  // second query tile sees kept positions also in the tiles between the two windows' first tiles (a tile of which
+  // it sees nothing is masked whole: at most one).
+  const int keep = p.window_kind == 2 ? p.keep_first : 0;
+  const int n_kept = min((keep + BKV - 1) / BKV, kb_phys[0]);
+  const int gap = kb_phys[0] - n_kept;
+  // exact tiles of A, then earlier blocks' tiles up to the one that holds the last position before A's (B's) last
+  // row's block, then exact tiles of B
+  const int first_exact[2] = {p0_x[0] / BKV, p0_x[1] / BKV};
+  const int n_exact[2] = {p1_x[0] / BKV - first_exact[0] + 1, has_b ? p1_x[1] / BKV - first_exact[1] + 1 : 0};
+  auto tiles_to = [&](int x) { return max((p1_x[x] / PAGE * PAGE + BKV - 1) / BKV - gap, 0); };
+  const int n_earlier = tiles_to(has_b ? 1 : 0);
+  int kb_x[2] = {0, n_exact[0] + (has_b && keep == 0 ? kb_phys[1] - gap : 0)};
+  int ke_x[2] = {n_exact[0] + tiles_to(0), has_b ? n_exact[0] + n_earlier + n_exact[1] : 0};
+  int kt0 = 0, kt1 = has_b ? ke_x[1] : ke_x[0];                           // the union: every tile in it is met by A or B
+  if (p.n_splits > 1) {                                        // this block's share of the union
+    const int per = (kt1 + p.n_splits - 1) / p.n_splits;
+    kt0 = min(kt1, (int)blockIdx.z * per);
+    kt1 = min(kt1, kt0 + per);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) { kb_x[x] = min(max(kb_x[x], kt0), kt1); ke_x[x] = max(min(ke_x[x], kt1), kb_x[x]); }
+  }
+  auto is_exact = [&](int kt) { return kt < n_exact[0] || kt >= n_exact[0] + n_earlier; };
+  auto key_tile = [&](int kt) {
+    if (kt < n_exact[0]) return first_exact[0] + kt;
+    kt -= n_exact[0];
+    if (kt >= n_earlier) return first_exact[1] + kt - n_earlier;
+    return kt < n_kept ? kt : kt + gap;
+  };
+  const uint32_t tmem_s = tmem_base_s, tmem_o = tmem_base_s + 256;        // + 128 for tile B, both
+  volatile int* abort_flag = &abort_s;
+  bool ok = true;
+
+  if (warp == kSoftmaxWarps) {
+    if (lane == 0) {
+      // ---- TMA producer: Q of both tiles, then K(kt0), V(kt0), K(kt0 + 1), ... through the ring ----
+      mbar_expect_tx(&q_full, Q_BYTES * (has_b ? 2 : 1));
+      for (int x = 0; x < (has_b ? 2 : 1); ++x)
+        for (int h = 0; h < HALVES; ++h)
+          tma_load_2d(q_s + x * Q_BYTES + h * HALF_BYTES, &map_q, &q_full, head * D + h * 64, tok0 + x * BQ);
+      int n = 0;                                         // item of the ring: 2 (kt - kt0) for keys, + 1 for values
+      for (int kt = kt0; kt < kt1 && ok; ++kt) {
+        const int blk0 = key_tile(kt) * (BKV / PAGE);
+        const int* pages = (is_exact(kt) ? p.exact_table : p.earlier_table) + (size_t)seq * p.width;
+        for (int which = 0; which < 2; ++which, ++n) {
+          const int s = n % NSLOT;
+          if (n >= NSLOT && !mbar_wait(&kv_empty[s], ((n / NSLOT) - 1) & 1, abort_flag)) { ok = false; break; }
+          mbar_expect_tx(&kv_full[s], KV_BYTES);
+          for (int pg = 0; pg < BKV / PAGE; ++pg) {
+            int page = blk0 + pg < p.width ? pages[blk0 + pg] : -1;
+            if (page < 0 || page >= p.n_pages) page = p.n_pages;       // a page that the step does not have: beyond the tensor, zeros
+            const int row = (page * p.n_kv_heads + kvh) * PAGE;
+            for (int h = 0; h < HALVES; ++h)
+              tma_load_2d(ring + s * KV_BYTES + h * HALF_BYTES + pg * (PAGE * 128), which ? &map_v : &map_k,
+                          &kv_full[s], h * 64, row);
+          }
+        }
+      }
+    }
+  } else if (warp == kSoftmaxWarps + 1) {
+    // ---- MMA issuer.  Two query tiles share every key and value tile.  Per key tile kt:
+    //          O_A += P_A V(kt);  S_A = Q_A K(kt+1)^T;   O_B += P_B V(kt);  S_B = Q_B K(kt+1)^T
+    //      so that while the softmax threads of one query tile work on its S, the tensor pipe runs the other
+    //      tile's products.  P is written over the S it came from (as bf16, the first 64 columns) and is the
+    //      A operand of P V from tensor memory; the next Q K^T of the same query tile is issued after that
+    //      P V and the pipe runs in issue order, so it cannot overwrite a P that is still being read.
+    //      The whole warp runs the loop (uniform values stay on the uniform datapath); only the tcgen05
+    //      instructions sit under the elected lane. ----
+    constexpr uint32_t idesc_s = instr_desc(BQ, BKV, 0);
+    constexpr uint32_t idesc_o = instr_desc(BQ, D, 1);
+    constexpr uint64_t kSlotUnits = KV_BYTES >> 4;      // a ring slot further, in the descriptor's 16-byte units
+    const uint64_t dq[2] = {smem_desc(smem_u32(q_s), 16, 1024), smem_desc(smem_u32(q_s + Q_BYTES), 16, 1024)};
+    const uint64_t dk0 = smem_desc(smem_u32(ring), 16, 1024), dv0 = smem_desc(smem_u32(ring), HALF_BYTES, 1024);
+    // Everything the loop needs is a counter that is advanced by additions (this warp shares its scheduler with
+    // two softmax warps: every instruction between two MMAs is time the tensor pipe stands still).  Ring slot
+    // and phase of the next key tile and of the next value tile to be used, per query tile:
+    int ks[2], kph[2], vs[2], vph[2], pph[2] = {0, 0}, first_pv[2] = {1, 1};
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int nk = 2 * (kb_x[x] - kt0), nv = nk + 1;
+      ks[x] = nk % NSLOT; kph[x] = (nk / NSLOT) & 1;
+      vs[x] = nv % NSLOT; vph[x] = (nv / NSLOT) & 1;
+    }
+    // S_x = Q_x K^T on the key tile in ring slot ks[x]; `release`: no later product reads that key tile
+    auto issue_qk = [&](int x, bool release) -> bool {
+      if (!__all_sync(0xffffffffu, mbar_wait(&kv_full[ks[x]], kph[x], abort_flag))) return false;
+      fence_after_sync();
+      if (elect_one()) {
+        const uint64_t dk = dk0 + (uint64_t)ks[x] * kSlotUnits;
+        umma_bf16_c<false>(tmem_s + x * 128, dq[x], dk, idesc_s);
+#pragma unroll
+        for (int k = 1; k < D / 16; ++k) {
+          const uint64_t off = (uint64_t)(((k >> 2) * HALF_BYTES + (k & 3) * 32) >> 4);
+          umma_bf16_c<true>(tmem_s + x * 128, dq[x] + off, dk + off, idesc_s);
+        }
+        umma_commit(&s_full[x]);
+        if (release) umma_commit(&kv_empty[ks[x]]);
+      }
+      __syncwarp();
+      ks[x] += 2;                                        // the next key tile is two ring items further
+      if (ks[x] >= NSLOT) { ks[x] -= NSLOT; kph[x] ^= 1; }
+      return true;
+    };
+    // O_x += P_x V on the value tile in ring slot vs[x]
+    auto issue_pv = [&](int x, bool release) -> bool {
+      if (!__all_sync(0xffffffffu, mbar_wait(&p_full[x], pph[x], abort_flag) &&
+                                       mbar_wait(&kv_full[vs[x]], vph[x], abort_flag))) return false;
+      fence_after_sync();
+      if (elect_one()) {
+        const uint64_t dv = dv0 + (uint64_t)vs[x] * kSlotUnits;
+        const uint32_t pa = tmem_s + x * 128, od = tmem_o + x * 128;
+        if (first_pv[x]) umma_bf16_a_tmem_c<false>(od, pa, dv, idesc_o);
+        else umma_bf16_a_tmem_c<true>(od, pa, dv, idesc_o);
+#pragma unroll
+        for (int j = 1; j < BKV / 16; ++j)
+          umma_bf16_a_tmem_c<true>(od, pa + j * 8, dv + (uint64_t)(j * (2048 >> 4)), idesc_o);
+        if (release) umma_commit(&kv_empty[vs[x]]);
+      }
+      __syncwarp();
+      first_pv[x] = 0;
+      pph[x] ^= 1;
+      vs[x] += 2;
+      if (vs[x] >= NSLOT) { vs[x] -= NSLOT; vph[x] ^= 1; }
+      return true;
+    };
+    ok = __all_sync(0xffffffffu, mbar_wait(&q_full, 0, abort_flag));
+    // (a share of the union may have nothing for A, or nothing for B)
+    const int kb_b = has_b && kb_x[1] < ke_x[1] ? kb_x[1] : 0x7fffffff, ke_a = ke_x[0];
+    if (ke_a > kt0) ok = ok && issue_qk(0, kb_b != kt0);
+    if (ok && kb_b == kt0) ok = issue_qk(1, true);
+    for (int kt = kt0; kt < kt1 && ok; ++kt) {
+      // which query tiles meet key tile kt, and kt + 1 (B's range ends with the union's, A's begins with it)
+      const bool a_now = kt < ke_a, b_now = kt >= kb_b;
+      const bool a_next = kt + 1 < ke_a, b_next = kt + 1 >= kb_b && kt + 1 < kt1;
+      if (a_now) {
+        ok = issue_pv(0, !b_now);
+        if (ok && a_next) ok = issue_qk(0, !b_next);
+      }
+      if (ok && b_now) ok = issue_pv(1, true);
+      if (ok && b_next) ok = issue_qk(1, true);
+    }
+    // every product has been issued: one arrival says that O of both query tiles is complete
+    if (ok && elect_one()) { umma_commit(&o_done[0]); umma_commit(&o_done[1]); }
+    __syncwarp();
+  } else {
+    // ---- softmax: warps 0-3 own query tile A, warps 4-7 tile B; thread r of a group owns query row r and all
+    //      128 key columns of a tile (a warp may touch the 32 lanes of tensor memory given by its number modulo
+    //      4).  Row maxima and sums need no shuffles.  O stays in tensor memory and is rescaled only when a row maximum has
+    //      outgrown its reference. ----
+    const int x = warp >> 2, row = tid & 127;
+    const bool live = row < rows_x[x];
+    const int qp = live ? p0_x[x] + row : -1;
+    const int lo = live ? window_low(p.window_kind, p.window_size, qp) : 0;
+    const int lo_last = window_low(p.window_kind, p.window_size, p1_x[x]);
+    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_row = tmem_s + x * 128 + lane_addr, o_row = tmem_o + x * 128 + lane_addr;
+    float m_ref = -1e30f, l_run = 0.f;                  // reference maximum of the exponentials; the row's sum
+    // > 0: the maximum may be taken before scaling.  Under a soft cap c a raw score s first becomes tanh(s scale / c)
+    // (monotonic too) and the factor is c log2(e)
+    const float sc = CAPPED ? p.cap_out : p.scale_log2, cap_in = p.cap_in;
+    const int edge = live ? qp / PAGE * PAGE : 0;       // the row's own block begins here
+    const int edge_first = p0_x[x] / PAGE * PAGE;
+    int j = 0;
+    bool okl = rows_x[x] > 0;
+    for (int kt = kb_x[x]; kt < ke_x[x] && okl; ++kt, ++j) {
+      const int key0 = key_tile(kt) * BKV;
+      const bool exact = is_exact(kt);
+      // (tensor-memory loads and votes are warp-wide: a warp gives up as a whole)
+      okl = __all_sync(0xffffffffu, mbar_wait(&s_full[x], j & 1, abort_flag));
+      if (!okl) break;
+      fence_after_sync();
+      // a tile that lies wholly inside every row's window, and before every row's block, needs no position tests
+      const bool no_mask = !exact && key0 + BKV <= edge_first && (key0 >= lo_last || key0 + BKV - 1 < keep);
+      auto sees = [&](int first) {
+        const int n = edge - first;
+        const uint32_t before = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+        return visible(qp, lo, keep, first) & (exact ? ~before : before);
+      };
+      bool stored = false;
+      if (!CAPPED && no_mask && j > 0) {
+        uint32_t w[BKV / 32][16], raw[BKV / 32][32];
+        const float nref = -m_ref;
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, ls4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int cc = 0; cc < BKV / 32; ++cc) tmem_ld32_issue(s_row + cc * 32, raw[cc]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int cc = 0; cc < BKV / 32; ++cc) {
+          float v[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float sv = __uint_as_float(raw[cc][e]);
+            mx4[e & 3] = fmaxf(mx4[e & 3], sv);
+            v[e] = exp2_fast(fmaf(sv, sc, nref));
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) ls4[e & 3] += v[e];
+#pragma unroll
+          for (int g = 0; g < 16; ++g) w[cc][g] = pack_bf16(v[2 * g], v[2 * g + 1]);
+        }
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+        stored = !__any_sync(0xffffffffu, mx > m_ref + (m_ref < -1e29f ? 0.f : kWideSlack));
+        if (stored) {
+#pragma unroll
+          for (int cc = 0; cc < BKV / 32; ++cc) tmem_st16_nowait(s_row + cc * 16, w[cc]);
+          l_run += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
+        }
+      }
+      if (!stored) {
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < BKV; c += 32) {
+          const uint32_t in = no_mask ? 0xffffffffu : sees(key0 + c);
+          if (!__any_sync(0xffffffffu, in != 0)) continue;
+          float v[32], mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          tmem_ld32(s_row + c, v);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], (in >> e) & 1u ? v[e] : -INFINITY);
+          mx = fmaxf(mx, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
+        }
+        mx = CAPPED && mx > -INFINITY ? tanh_fast(mx * cap_in) * sc : mx * sc;
+        const bool grow = mx > m_ref + (m_ref < -1e29f ? 0.f : kWideSlack);
+        if (j == 0) {
+          m_ref = fmaxf(mx, m_ref);
+        } else if (__any_sync(0xffffffffu, grow)) {
+          const float m_new = grow ? mx : m_ref, f = exp2f(m_ref - m_new);
+          // Every P V issued so far for this query tile has landed: the Q K^T whose S was waited for above was issued after the
+          // last of them, and its arrival covers everything issued before it.
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            float v[32];
+            tmem_ld32(o_row + c, v);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] *= f;
+            tmem_st32(o_row + c, v);
+          }
+          l_run *= f;
+          m_ref = m_new;
+        }
+        const float nref = -m_ref;
+#pragma unroll 1
+        for (int c = 0; c < BKV; c += 32) {
+          const uint32_t in = no_mask ? 0xffffffffu : sees(key0 + c);
+          uint32_t w[16] = {};
+          if (__any_sync(0xffffffffu, in != 0)) {
+            float v[32], ls4[4] = {0.f, 0.f, 0.f, 0.f};
+            tmem_ld32(s_row + c, v);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              if (CAPPED) v[e] = tanh_fast(v[e] * cap_in);
+              v[e] = (in >> e) & 1u ? exp2_fast(fmaf(v[e], sc, nref)) : 0.f;
+              ls4[e & 3] += v[e];
+            }
+#pragma unroll
+            for (int g = 0; g < 16; ++g) w[g] = pack_bf16(v[2 * g], v[2 * g + 1]);
+            l_run += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
+          }
+          tmem_st16_nowait(s_row + (c >> 1), w);
+        }
+      }
+      tmem_wait_st();
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[x]);            // one arrival per warp
+    }
+    // the output: O / l once the last P V is done
+    ok = okl && !abort_s && j > 0;
+    const size_t at = (size_t)(tok0 + x * BQ + row) * p.n_heads + head;
+    if (p.n_splits > 1 && live) {
+      // what this share adds up to: the row's sum and what it is measured against (nothing: a sum of zero)
+      p.part_ml[at * p.n_splits + blockIdx.z] = make_float2(m_ref, j > 0 ? l_run : 0.f);
+    }
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(&o_done[x], 0, abort_flag));
+    fence_after_sync();
+    if (ok) {
+      if (p.n_splits > 1) {
+        float* dst = p.part_o + (at * p.n_splits + blockIdx.z) * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float v[32];
+          tmem_ld32(o_row + c, v);
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(dst + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          }
+        }
+      } else {
+        // a sink adds 2^(sink log2 e - reference) to the row's sum and nothing to O; the exponent is capped so that a
+        // sink far above every score gives a huge finite sum
+        if (p.sink) l_run += exp2f(fminf(p.sink[head] * 1.4426950408889634f - m_ref, 120.f));
+        const float inv = 1.0f / fmaxf(l_run, 1e-20f);
+        __nv_bfloat16* dst = p.out + at * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float v[32];
+          tmem_ld32(o_row + c, v);
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(pack_bf16(v[e] * inv, v[e + 1] * inv), pack_bf16(v[e + 2] * inv, v[e + 3] * inv),
+                                                                  pack_bf16(v[e + 4] * inv, v[e + 5] * inv), pack_bf16(v[e + 6] * inv, v[e + 7] * inv));
+          }
+        }
+      }
+    }
+    fence_before_sync();
+  }
+  if (abort_s) {
+    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 2);
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_s), "r"(TMEM_COLS));
+}
+
+// The shares of a query tile's keys joined: out[t, h] = sum_s w_s O_s / (sum_s w_s l_s + sink), w_s = 2^(m_s - max m).  A warp per
+// (token, head), four features or two per lane.
+template <int D>
+__global__ void __launch_bounds__(256) attention_prefill_combine(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
+                                                                 __nv_bfloat16* __restrict__ out, long rows, int n_splits,
+                                                                 const float* __restrict__ sink, int n_heads) {
+  constexpr int PER = D / 32;
+  const int lane = threadIdx.x & 31;
+  const long th = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (th >= rows) return;
+  const float2 ml = lane < n_splits ? __ldcg(part_ml + th * n_splits + lane) : make_float2(-1e30f, 0.f);
+  const float M = warp_max(ml.x);
+  const float w = exp2f(ml.x - M), l = ml.y > 0.f || ml.y != ml.y ? w * ml.y : 0.f;
+  float L = warp_sum(l), acc[PER] = {};
+  for (int s = 0; s < n_splits; ++s) {
+    const float ws = __shfl_sync(0xffffffffu, w, s), ls = __shfl_sync(0xffffffffu, ml.y, s);
+    if (ls == 0.f) continue;                             // (this share held nothing for the row, or was not written)
+    const float* src = part_o + (th * n_splits + s) * D + lane * PER;
+    if (PER == 4) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+      acc[0] += ws * v.x; acc[1] += ws * v.y; acc[PER - 2] += ws * v.z; acc[PER - 1] += ws * v.w;
+    } else {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+      acc[0] += ws * v.x; acc[1] += ws * v.y;
+    }
+  }
+  if (sink) L += exp2f(fminf(sink[th % n_heads] * 1.4426950408889634f - M, 120.f));
+  const float inv = 1.0f / fmaxf(L, 1e-20f);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(out + th * D + lane * PER);
+#pragma unroll
+  for (int i = 0; i < PER / 2; ++i) dst[i] = pack_bf16(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+}
+
+}  // namespace pre8
+}  // namespace cpi
+
+using namespace cpi;
+
+// q, out [T, NH*D] bfloat16; k_pages, v_pages [n_pages, NKV, 64, D] bfloat16, named per sequence of the
+// step and block by earlier_table and exact_table [sequences, width] (-1: none).  `n_splits` > 1: that many blocks of threads share a query tile's
+// keys, through `scratch` (n_tokens * n_heads * n_splits * (head_dim + 2) floats).
+extern "C" int cpi_attention_prefill_kv8(const void* q, void* out, const void* k_pages, const void* v_pages, long n_pages,
+                                         const int* earlier_table, const int* exact_table, int n_seqs, int width, const int* token_seq,
+                                         const int* token_pos, const int* tile_tok0, const int* tile_rows, int n_tiles, int n_tokens,
+                                         int n_heads, int n_kv_heads, int head_dim, int window_kind, int window_size, int keep_first,
+                                         float scale, float softcap, const float* sink, int n_splits, float* scratch, int* error_flag,
+                                         cudaStream_t stream) {
+  if (n_tiles == 0 || n_tokens == 0) return 0;
+  const long rows = (long)n_tokens * n_heads;
+  CPI_REQUIRE(n_splits >= 1 && n_splits <= 32 && (n_splits == 1 || scratch), "attention_prefill_kv8: %d shares (up to 32, with scratch)", n_splits);
+  CPI_REQUIRE(n_kv_heads >= 1 && n_heads % n_kv_heads == 0 && (head_dim == 64 || head_dim == 128),
+              "attention_prefill_kv8: unsupported shape (heads %d/%d, head size %d)", n_heads, n_kv_heads, head_dim);
+  CPI_REQUIRE(window_kind == 0 || window_size > 0, "attention_prefill_kv8: window kind %d needs a size > 0", window_kind);
+  CPI_REQUIRE(n_tiles <= 65535, "attention_prefill_kv8: too many query tiles in one launch (%d)", n_tiles);
+  const uint64_t kv_rows = (uint64_t)n_pages * n_kv_heads * pre8::PAGE;
+  CPI_REQUIRE(n_pages > 0 && kv_rows + (uint64_t)n_kv_heads * pre8::PAGE < (1ull << 31), "attention_prefill_kv8: %ld pages of %d heads", n_pages, n_kv_heads);
+  CUtensorMap mq, mk, mv;
+  const uint64_t q_width = (uint64_t)n_heads * head_dim;
+  if (tc::get_map_2d_bf16(q, q_width, (uint64_t)n_tokens, q_width * 2, 64, pre::BQ, &mq)) return 1;
+  if (tc::get_map_2d_bf16(k_pages, (uint64_t)head_dim, kv_rows, (uint64_t)head_dim * 2, 64, pre8::PAGE, &mk)) return 1;
+  if (tc::get_map_2d_bf16(v_pages, (uint64_t)head_dim, kv_rows, (uint64_t)head_dim * 2, 64, pre8::PAGE, &mv)) return 1;
+  pre8::Params p{(__nv_bfloat16*)out, earlier_table, exact_table, width, token_pos, token_seq, tile_tok0, tile_rows,
+                n_heads, n_kv_heads, window_kind, window_size, keep_first > 0 ? keep_first : 0, scale * 1.4426950408889634f, error_flag, sink,
+                softcap > 0.f ? scale / softcap : 0.f, softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, (int)n_pages, n_tokens, n_seqs, n_splits, scratch,
+                scratch ? reinterpret_cast<float2*>(scratch + rows * n_splits * head_dim) : nullptr};
+  dim3 grid(n_heads, n_tiles, n_splits);
+  // One block of threads to an SM: each takes all of the tensor memory.  Two heads' worth of 64 would fit an SM's shared memory, and
+  // a second block that is put there, while the kernel before still fills the other SMs, waits for the first to end (four windowed
+  // prompts, 144 blocks: 80 us instead of 47).
+  const int smem = head_dim == 64 ? 120 * 1024 : head_dim / 64 * 128 * 128 * (2 + pre8::kRingSlots);
+  auto launch = [&](auto dim, auto capped) {
+    auto* kernel = pre8::attention_prefill_kv8_kernel<dim.value, capped.value>;
+    static bool set[64] = {};                              // per device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !set[dev]) {
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (dev >= 0 && dev < 64) set[dev] = true;
+    }
+    cpi::launch_pdl(kernel, grid, pre8::kThreads, smem, stream, mq, mk, mv, p);
+  };
+  auto launch_dim = [&](auto dim) {
+    if (p.cap_out > 0.f) launch(dim, std::true_type{}); else launch(dim, std::false_type{});
+  };
+  if (head_dim == 128) launch_dim(std::integral_constant<int, 128>{}); else launch_dim(std::integral_constant<int, 64>{});
+  if (check_launch("attention_prefill_kv8")) return 2;
+  if (n_splits == 1) return 0;
+  auto* combine = head_dim == 128 ? pre8::attention_prefill_combine<128> : pre8::attention_prefill_combine<64>;
+  cpi::launch_pdl(combine, dim3((unsigned)((rows + 7) / 8)), 256, 0, stream, p.part_o, p.part_ml, p.out, rows, n_splits, sink, n_heads);
+  return check_launch("attention_prefill_combine");
+}
+CPI_PACKED(cpi_attention_prefill_kv8)

@@ -10,6 +10,7 @@
 //                   tail before (the sequence's first own block), so no other block of threads can still want the old rows
 // Bound by bytes: an earlier block reads 1 byte and writes 2 per element, an own block reads 2 and writes 3.
 #include "kv8.cuh"
+#include "packed.cuh"
 
 namespace cpi {
 namespace kv8 {
@@ -124,3 +125,4 @@ extern "C" int cpi_kv8_stage(const int* jobs, int n_jobs, const int* page_table,
   cpi::launch_pdl(kernel, grid, 256, 0, stream, p);
   return check_launch("kv8_stage");
 }
+CPI_PACKED(cpi_kv8_stage)

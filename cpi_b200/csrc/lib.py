@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 from ctypes import c_int, c_long, c_float, c_void_p
 from typing import NamedTuple, Optional
 
@@ -1085,28 +1086,27 @@ def attention_decode(q, out, k_cache, v_cache, page_table, page_size, token_seq,
 
 
 # ---- the cache in 8 bits (see cpi_b200/cache/kv8.py for what it holds) ----------------------------------------------------
-# A call of these and of `log_probs` may take a few microseconds on the device, less than its own way there: arguments are declared
-# once (`_declared`), so that plain integers and floats go through without an object each, and checks read each tensor once.
-_INT, _LONG, _FLOAT, _PTR = c_int, c_long, c_float, c_void_p
+# A call of these and of `log_probs` may take a few microseconds on the device, less than its own way there: arguments go through in
+# one block of memory (see packed.cuh), and checks read each tensor once.
 _KV8_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
-
-
 _functions = {}
 
 
 def _declared(name: str, types: str):
-    """The library's function `name` with its arguments declared: p a pointer (int or None), i int, l long, f float."""
-    fn = _functions.get(name)
-    if fn is None:
-        fn = getattr(load(), name)
-        fn.argtypes = [{"p": _PTR, "i": _INT, "l": _LONG, "f": _FLOAT}[t] for t in types]
-        _functions[name] = fn
-    return fn
+    """(The library's function `name` that takes its arguments in one block, what packs them): of `types` p is an address (0:
+    none), i and l are integers, f is a float."""
+    found = _functions.get(name)
+    if found is None:
+        fn = getattr(load(), name + "_packed")
+        fn.argtypes = [ctypes.c_char_p]
+        found = _functions[name] = fn, struct.Struct("=" + "".join({"p": "Q", "i": "q", "l": "q", "f": "d"}[t] for t in types)).pack
+    return found
 
 
-def _run(fn, *args):
+def _run(declared, *args):
     global launch_count
-    if fn(*args):
+    fn, pack = declared
+    if fn(pack(*args)):
         raise KernelError(load().cpi_last_error().decode())
     launch_count += 1
 
@@ -1209,7 +1209,7 @@ def attention_decode_kv8(q, out, cache, page_table, token_seq, token_pos, seq_sl
     fmt, nkv, d, slots, at = _kv8(cache, what, n_heads)
     T, table = q.shape[0], page_table.shape
     here = _here(what, q, out, page_table, token_seq, token_pos, seq_slot, *cache)
-    sink_at = None
+    sink_at = 0
     if sink is not None:
         _here(what, q, sink)
         sink_at = sink.data_ptr()
@@ -1228,7 +1228,7 @@ def attention_decode_kv8(q, out, cache, page_table, token_seq, token_pos, seq_sl
     scratch = torch.empty(T * n_heads * splits * (d + 2), dtype=torch.float32, device=q.device) if joined else None
     _run(_declared("cpi_attention_decode_kv8", "ppppppippipipppiiiiiiiiiffpippp"), q_at, out_at, at[0], at[1], at[2], at[3], cache[0].shape[0],
          at[4], at[5], slots, table_at, table[1], seq_at, pos_at, slot_at, seq_slot.numel(), T, n_heads, nkv, d, fmt, window_kind, window_size,
-         keep_first, scale, softcap or 0.0, sink_at, splits, scratch.data_ptr() if joined else None, _flag(here), _raw_stream(here))
+         keep_first, scale, softcap or 0.0, sink_at, splits, scratch.data_ptr() if joined else 0, _flag(here), _raw_stream(here))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1271,7 +1271,7 @@ def attention_prefill_kv8(q, out, k_pages, v_pages, plan, token_seq, token_pos, 
     if n_heads < 1 or nkv < 1 or n_heads % nkv:
         raise KernelError(f"{what}: {n_heads} query heads over {nkv} key/value heads")
     here = _here(what, q, out, k_pages, v_pages, plan.jobs, token_seq, token_pos, tile_tok0, tile_rows)
-    sink_at = None
+    sink_at = 0
     if sink is not None:
         _here(what, q, sink)
         sink_at = sink.data_ptr()
@@ -1289,7 +1289,7 @@ def attention_prefill_kv8(q, out, k_pages, v_pages, plan, token_seq, token_pos, 
     _run(_declared("cpi_attention_prefill_kv8", "pppplppiippppiiiiiiiiffpippp"), q_at, out_at, k_at, v_at, plan.n_pages,
          plan.earlier_table.data_ptr(), plan.exact_table.data_ptr(), plan.n_seqs, plan.width, seq_at, pos_at, tok0_at, rows_at, tiles,
          plan.n_tokens, n_heads, nkv, d, window_kind, window_size, keep_first, scale, softcap or 0.0, sink_at, splits,
-         None if scratch is None else scratch.data_ptr(), _flag(here), _raw_stream(here))
+         0 if scratch is None else scratch.data_ptr(), _flag(here), _raw_stream(here))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1571,5 +1571,5 @@ def log_probs(logits, targets, *, top=0):
     if R:
         _run(_declared("cpi_log_probs", "piliipiippppip"), logits.data_ptr(), dtype_code(logits.dtype), logits.stride(0), R, V, targets.data_ptr(),
              1 if targets.dim() == 1 else targets.shape[1], int(targets.dtype is torch.int64), out.logprob.data_ptr(), out.entropy.data_ptr(),
-             out.top_logprobs.data_ptr() if top else None, out.top_ids.data_ptr() if top else None, top, _raw_stream(here))
+             out.top_logprobs.data_ptr() if top else 0, out.top_ids.data_ptr() if top else 0, top, _raw_stream(here))
     return out

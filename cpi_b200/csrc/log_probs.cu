@@ -20,6 +20,7 @@
 // probabilities -inf, entropy 0.  A row that holds NaN or +inf: log probabilities and entropy are NaN; NaN is never among the
 // best.  A target below zero stands for none (0 is returned), one beyond the vocabulary gives NaN.
 #include "common.cuh"
+#include "packed.cuh"
 
 namespace cpi {
 namespace lp {
@@ -531,3 +532,4 @@ extern "C" int cpi_log_probs(const void* logits, int dtype, long stride, int row
   set_error("log_probs: unknown dtype code %d", dtype);
   return 1;
 }
+CPI_PACKED(cpi_log_probs)
