@@ -25,9 +25,11 @@
 // threads meets most of this code cold, and one pass for all cases was more than an instruction cache holds.  Columns that no row of
 // the warp sees are passed over.
 //
-// Bound by the chain S -> softmax -> P V -> next S of each query tile, 4,400 cycles for two tiles of 128 x 128, where the products
-// take 2,048 and the exponentials as many.  Two threads to a row (sixteen warps) did not shorten it: with 96 registers a thread
-// either spills (238 us for 3,001 tokens of 40 heads) or reads S twice (168), against 155.
+// Bound by the chain S -> softmax -> P V -> next S of each query tile: about 4,100 cycles for two tiles of 128 x 128, where the
+// products take 2,048 and the exponentials as many.  3,001 tokens of 40/8 heads of 128: 149 us (620 TFLOP/s; the tensor pipe
+// stands still half of the time).  What was tried beside it: two threads to a row, sixteen warps, either spill with 96 registers each (238
+// us) or read S twice (168); a quarter of the exponentials as polynomials 160; waiting for the next tiles after P instead of before
+// it 155; without the look that does not suspend (wait_soon) 157.
 //
 // Few query tiles over many keys share their key tiles out among blocks of threads (n_splits), joined by a second kernel.
 // Every mbarrier wait is bounded; when one runs out the block sets *error_flag and leaves.
@@ -61,6 +63,13 @@ struct Params {
   float* part_o; float2* part_ml;     // with several: [T, NH, splits, D] sums, [T, NH, splits] reference and row sum
 };
 
+// As mbar_wait, with one look that does not suspend the thread first.
+__device__ __forceinline__ bool wait_soon(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0 || mbar_wait(bar, parity, abort_flag);
+}
 template <int D, bool CAPPED>
 __global__ void __launch_bounds__(kThreads, 1) attention_prefill_kv8_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                          const __grid_constant__ CUtensorMap map_k,
@@ -192,7 +201,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_prefill_kv8_kernel(cons
     //      so that while the softmax threads of one query tile work on its S, the tensor pipe runs the other
     //      tile's products.  P is written over the S it came from (as bf16, the first 64 columns) and is the
     //      A operand of P V from tensor memory; the next Q K^T of the same query tile is issued after that
-    //      P V and the pipe runs in issue order, so it cannot overwrite a P that is still being read.
+    //      P V and the pipe runs in issue order, so it cannot overwrite a P that is still being read.  What is still to be waited
+    //      for once P is there would leave the pipe idle between the two: the tiles are waited for before.
     //      The whole warp runs the loop (uniform values stay on the uniform datapath); only the tcgen05
     //      instructions sit under the elected lane. ----
     constexpr uint32_t idesc_s = instr_desc(BQ, BKV, 0);
@@ -200,73 +210,81 @@ __global__ void __launch_bounds__(kThreads, 1) attention_prefill_kv8_kernel(cons
     constexpr uint64_t kSlotUnits = KV_BYTES >> 4;      // a ring slot further, in the descriptor's 16-byte units
     const uint64_t dq[2] = {smem_desc(smem_u32(q_s), 16, 1024), smem_desc(smem_u32(q_s + Q_BYTES), 16, 1024)};
     const uint64_t dk0 = smem_desc(smem_u32(ring), 16, 1024), dv0 = smem_desc(smem_u32(ring), HALF_BYTES, 1024);
-    // Everything the loop needs is a counter that is advanced by additions (this warp shares its scheduler with
-    // two softmax warps: every instruction between two MMAs is time the tensor pipe stands still).  Ring slot
-    // and phase of the next key tile and of the next value tile to be used, per query tile:
-    int ks[2], kph[2], vs[2], vph[2], pph[2] = {0, 0}, first_pv[2] = {1, 1};
+    int ks = 0, kph = 0, vs = 1, vph = 0, pph[2] = {0, 0}, first_pv[2] = {1, 1};      // ring slots and phases of the next K and V
+    auto qk = [&](int x) {                              // (the elected lane) S_x = Q_x K^T on the key tile in slot ks
+      const uint64_t dk = dk0 + (uint64_t)ks * kSlotUnits;
+      umma_bf16_c<false>(tmem_s + x * 128, dq[x], dk, idesc_s);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int nk = 2 * (kb_x[x] - kt0), nv = nk + 1;
-      ks[x] = nk % NSLOT; kph[x] = (nk / NSLOT) & 1;
-      vs[x] = nv % NSLOT; vph[x] = (nv / NSLOT) & 1;
-    }
-    // S_x = Q_x K^T on the key tile in ring slot ks[x]; `release`: no later product reads that key tile
-    auto issue_qk = [&](int x, bool release) -> bool {
-      if (!__all_sync(0xffffffffu, mbar_wait(&kv_full[ks[x]], kph[x], abort_flag))) return false;
-      fence_after_sync();
-      if (elect_one()) {
-        const uint64_t dk = dk0 + (uint64_t)ks[x] * kSlotUnits;
-        umma_bf16_c<false>(tmem_s + x * 128, dq[x], dk, idesc_s);
-#pragma unroll
-        for (int k = 1; k < D / 16; ++k) {
-          const uint64_t off = (uint64_t)(((k >> 2) * HALF_BYTES + (k & 3) * 32) >> 4);
-          umma_bf16_c<true>(tmem_s + x * 128, dq[x] + off, dk + off, idesc_s);
-        }
-        umma_commit(&s_full[x]);
-        if (release) umma_commit(&kv_empty[ks[x]]);
+      for (int k = 1; k < D / 16; ++k) {
+        const uint64_t off = (uint64_t)(((k >> 2) * HALF_BYTES + (k & 3) * 32) >> 4);
+        umma_bf16_c<true>(tmem_s + x * 128, dq[x] + off, dk + off, idesc_s);
       }
-      __syncwarp();
-      ks[x] += 2;                                        // the next key tile is two ring items further
-      if (ks[x] >= NSLOT) { ks[x] -= NSLOT; kph[x] ^= 1; }
-      return true;
+      umma_commit(&s_full[x]);
     };
-    // O_x += P_x V on the value tile in ring slot vs[x]
-    auto issue_pv = [&](int x, bool release) -> bool {
-      if (!__all_sync(0xffffffffu, mbar_wait(&p_full[x], pph[x], abort_flag) &&
-                                       mbar_wait(&kv_full[vs[x]], vph[x], abort_flag))) return false;
-      fence_after_sync();
-      if (elect_one()) {
-        const uint64_t dv = dv0 + (uint64_t)vs[x] * kSlotUnits;
-        const uint32_t pa = tmem_s + x * 128, od = tmem_o + x * 128;
-        if (first_pv[x]) umma_bf16_a_tmem_c<false>(od, pa, dv, idesc_o);
-        else umma_bf16_a_tmem_c<true>(od, pa, dv, idesc_o);
+    auto pv = [&](int x) {                              // (the elected lane) O_x += P_x V on the value tile in slot vs
+      const uint64_t dv = dv0 + (uint64_t)vs * kSlotUnits;
+      const uint32_t pa = tmem_s + x * 128, od = tmem_o + x * 128;
+      if (first_pv[x]) umma_bf16_a_tmem_c<false>(od, pa, dv, idesc_o);
+      else umma_bf16_a_tmem_c<true>(od, pa, dv, idesc_o);
 #pragma unroll
-        for (int j = 1; j < BKV / 16; ++j)
-          umma_bf16_a_tmem_c<true>(od, pa + j * 8, dv + (uint64_t)(j * (2048 >> 4)), idesc_o);
-        if (release) umma_commit(&kv_empty[vs[x]]);
-      }
-      __syncwarp();
-      first_pv[x] = 0;
-      pph[x] ^= 1;
-      vs[x] += 2;
-      if (vs[x] >= NSLOT) { vs[x] -= NSLOT; vph[x] ^= 1; }
-      return true;
+      for (int j = 1; j < BKV / 16; ++j) umma_bf16_a_tmem_c<true>(od, pa + j * 8, dv + (uint64_t)(j * (2048 >> 4)), idesc_o);
     };
-    ok = __all_sync(0xffffffffu, mbar_wait(&q_full, 0, abort_flag));
-    // (a share of the union may have nothing for A, or nothing for B)
+    auto landed = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, wait_soon(bar, parity, abort_flag)); };
+    auto further = [&](int& s, int& ph) { s += 2; if (s >= NSLOT) { s -= NSLOT; ph ^= 1; } };
+    // Which query tiles meet key tile kt (A a prefix of the axis, B a suffix; a share of it may have nothing for one of them).
     const int kb_b = has_b && kb_x[1] < ke_x[1] ? kb_x[1] : 0x7fffffff, ke_a = ke_x[0];
-    if (ke_a > kt0) ok = ok && issue_qk(0, kb_b != kt0);
-    if (ok && kb_b == kt0) ok = issue_qk(1, true);
-    for (int kt = kt0; kt < kt1 && ok; ++kt) {
-      // which query tiles meet key tile kt, and kt + 1 (B's range ends with the union's, A's begins with it)
-      const bool a_now = kt < ke_a, b_now = kt >= kb_b;
-      const bool a_next = kt + 1 < ke_a, b_next = kt + 1 >= kb_b && kt + 1 < kt1;
-      if (a_now) {
-        ok = issue_pv(0, !b_now);
-        if (ok && a_next) ok = issue_qk(0, !b_next);
+    ok = landed(&q_full, 0);
+    if (kt0 < kt1) ok = ok && landed(&kv_full[ks], kph);
+    if (ok && kt0 < kt1) {
+      fence_after_sync();
+      if (elect_one()) {
+        if (ke_a > kt0) qk(0);
+        if (kb_b == kt0) qk(1);
+        umma_commit(&kv_empty[ks]);
       }
-      if (ok && b_now) ok = issue_pv(1, true);
-      if (ok && b_next) ok = issue_qk(1, true);
+      __syncwarp();
+      further(ks, kph);
+    }
+    for (int kt = kt0; kt < kt1 && ok; ++kt) {
+      const bool a_now = kt < ke_a, b_now = kt >= kb_b, last = kt + 1 == kt1;
+      const bool a_next = kt + 1 < ke_a, b_next = kt + 1 >= kb_b && !last;
+      ok = landed(&kv_full[vs], vph) && (last || landed(&kv_full[ks], kph));
+      if (ok && a_now) {
+        ok = landed(&p_full[0], pph[0]);
+        pph[0] ^= 1;
+        fence_after_sync();
+        if (ok && elect_one()) {
+          pv(0);
+          if (!b_now) umma_commit(&kv_empty[vs]);
+          if (a_next) {
+            qk(0);
+            if (!b_next) umma_commit(&kv_empty[ks]);
+          }
+        }
+        __syncwarp();
+        first_pv[0] = 0;
+      }
+      if (ok && (b_now || b_next)) {
+        if (b_now) {
+          ok = landed(&p_full[1], pph[1]);
+          pph[1] ^= 1;
+        }
+        fence_after_sync();
+        if (ok && elect_one()) {
+          if (b_now) {
+            pv(1);
+            umma_commit(&kv_empty[vs]);
+          }
+          if (b_next) {
+            qk(1);
+            umma_commit(&kv_empty[ks]);
+          }
+        }
+        __syncwarp();
+        if (b_now) first_pv[1] = 0;
+      }
+      further(ks, kph);
+      further(vs, vph);
     }
     // every product has been issued: one arrival says that O of both query tiles is complete
     if (ok && elect_one()) { umma_commit(&o_done[0]); umma_commit(&o_done[1]); }
@@ -295,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_prefill_kv8_kernel(cons
       const int key0 = key_tile(kt) * BKV;
       const bool exact = is_exact(kt);
       // (tensor-memory loads and votes are warp-wide: a warp gives up as a whole)
-      okl = __all_sync(0xffffffffu, mbar_wait(&s_full[x], j & 1, abort_flag));
+      okl = __all_sync(0xffffffffu, wait_soon(&s_full[x], j & 1, abort_flag));
       if (!okl) break;
       fence_after_sync();
       // a tile that lies wholly inside every row's window, and before every row's block, needs no position tests
