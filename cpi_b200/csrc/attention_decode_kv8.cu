@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kern
       }
     }
 
-    float ks_all = 0.f, vs_all = 0.f;
+    float ks_all = 0.f, ev_all = 0.f;
     int at = 0;                                             // the slot of the next tile
     uint32_t parity = 0;
     auto next = [&] { if (++at == SLOTS) { at = 0; parity ^= 1u; } };
@@ -439,10 +439,9 @@ __global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kern
         const int page = x + lane < mine ? table[block_at(x + lane)] : -1;
         const bool ok = page >= 0 && page < total_pages;
         ks_all = ok ? p.k_scale[(size_t)page * p.n_kv_heads + kvh] : 0.f;
-        vs_all = ok ? p.v_scale[(size_t)page * p.n_kv_heads + kvh] : 1.f;
+        ev_all = ok ? log2f(fmaxf(p.v_scale[(size_t)page * p.n_kv_heads + kvh], 1e-30f)) : 0.f;      // (any scale is good)
       }
-      const float ks = __shfl_sync(0xffffffffu, ks_all, x & 31), vs = __shfl_sync(0xffffffffu, vs_all, x & 31);
-      const int ev_i = (int)((__float_as_uint(vs) >> 23) & 0xffu) - 127;                  // vs = 2^ev_i
+      const float ks = __shfl_sync(0xffffffffu, ks_all, x & 31), ev = __shfl_sync(0xffffffffu, ev_all, x & 31);
       const int first = block_at(x) * PAGE + (half_of(x) & 1) * POS;
       const bool ragged = first < lo && first + POS - 1 >= keep;            // (every position of a complete block is before pos)
       if (!__all_sync(0xffffffffu, mbar_wait(&bars[at], parity, aborted))) break;
@@ -471,7 +470,7 @@ __global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kern
       __syncwarp();                                         // every lane has its keys (they are in products): the slot is free
       ask(2 * x + SLOTS, at);
       next();
-      const float ev = (float)ev_i, v_inv = kv8::power_of_two(-ev_i);
+      const float v_inv = ex2(-ev);                         // (exact for a power of two)
       float mx[HT][2];
 #pragma unroll
       for (int h = 0; h < HT; ++h)
@@ -796,7 +795,7 @@ extern "C" int cpi_attention_decode_kv8(const void* q, void* out, void* k, void*
   // the codes as lines of 128 bytes: a tile of 32 positions of a head is 32 * D / 128 of them
   CUtensorMap mk, mv;
   const uint64_t lines = (uint64_t)n_pages * n_kv_heads * (kv8::PAGE * head_dim / 128);
-  CPI_REQUIRE(n_pages > 0 && lines + kv8::PAGE < (1ull << 31), "attention_decode_kv8: a cache of %d pages of %d heads", n_pages, n_kv_heads);
+  CPI_REQUIRE(n_pages > 0 && lines + (uint64_t)n_kv_heads * kv8::PAGE < (1ull << 31), "attention_decode_kv8: a cache of %d pages of %d heads", n_pages, n_kv_heads);
   if (tc::get_map_2d_bf16(k, 64, lines, 128, 64, 32 * head_dim / 128, &mk)) return 1;
   if (tc::get_map_2d_bf16(v, 64, lines, 128, 64, 32 * head_dim / 128, &mv)) return 1;
   const long parts = (long)n_tokens * n_heads * n_splits;

@@ -284,6 +284,9 @@ class Engine:
             return
         self._err_dev.zero_()
         self._err_host.zero_()
+        if gave_up == 3:
+            raise RuntimeError("attention: a position, slot or page of a step was outside of the cache; the results of the steps since the "
+                               "last check are invalid")
         if gave_up:
             raise RuntimeError("a tensor-core kernel gave up waiting on one of its barriers; the results of the "
                                "steps since the last check are invalid")

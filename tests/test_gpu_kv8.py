@@ -176,12 +176,38 @@ def test_single_tokens_sink_and_cap(sink, softcap, max_context):
         rig.check(i, q[i:i + 1], out[i:i + 1], [p], sink=sink, softcap=softcap)
 
 
-def test_long_context_many_splits():
-    p = 9000
-    rig = Rig([p + 1], fmt="e4m3", nh=4, nkv=1, d=64, seed=5)
+@pytest.mark.parametrize("nh,d,splits", [(4, 64, s) for s in range(1, 10)] + [(5, 128, 3), (16, 128, 2), (12, 64, 7), (16, 128, 8), (8, 128, 17), (9, 128, 20),
+                                         (4, 64, 35)])
+def test_splits_of_the_keys(nh, d, splits):
+    """One block of threads, clusters of any size, and blocks that a second kernel joins, with few heads and with two tiles of them."""
+    p = (4 * splits - 1) * 64 - 7
+    assert K._kv8_splits(0, 1, -(-(p + 1) // 64))[0] == splits
+    rig = Rig([p + 1], fmt="e4m3", nh=nh, nkv=1, d=d, seed=5)
     rig.load(0, p)
+    sink = torch.linspace(-3, 9, nh, device=DEV) if splits % 2 else None
+    q, out = rig.decode([p], sink=sink)
+    rig.check(0, q, out, [p], sink=sink)
+
+
+def test_scales_that_are_no_powers_of_two():
+    """Codes of another maker: any positive scales."""
+    p = 200
+    rig = Rig([p + 1], nh=4, nkv=2, d=64, seed=31)
+    rig.load(0, p)
+    rig.cache.k_scale.mul_(1.37)
+    rig.cache.v_scale.mul_(0.71)
     q, out = rig.decode([p])
-    rig.check(0, q, out, [p])
+    held = {}
+    for name in ("k", "v"):
+        x = getattr(rig, name)[0].double()
+        for b in range(3):
+            page = int(rig.table[rig.slots[0], b])
+            codes, scales = getattr(rig.cache, name)[page].double(), getattr(rig.cache, name + "_scale")[page].double()
+            x[b * 64:(b + 1) * 64] = (codes * scales[:, None, None]).transpose(0, 1)
+        held[name] = x.repeat_interleave(2, 1)
+    s = torch.softmax(torch.einsum("hd,jhd->hj", q[0].double(), held["k"]) / 8.0, 1)
+    ref, mag = torch.einsum("hj,jhd->hd", s, held["v"]), torch.einsum("hj,jhd->hd", s, held["v"].abs())
+    assert ((out[0].double() - ref).abs() <= P.tolerance(ref, mag)).all()
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
