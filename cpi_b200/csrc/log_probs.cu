@@ -503,8 +503,8 @@ int launch(const Params& p, int rows, cudaStream_t stream) {
   return check_launch("log_probs");
 }
 template <typename T, bool TOP>
-int launch(const Params& p, int rows, bool wide, cudaStream_t stream) {
-  return wide ? launch<T, TOP, 512>(p, rows, stream) : launch<T, TOP, 256>(p, rows, stream);
+int launch(const Params& p, int rows, int threads, cudaStream_t stream) {
+  return threads == 512 ? launch<T, TOP, 512>(p, rows, stream) : threads == 256 ? launch<T, TOP, 256>(p, rows, stream) : launch<T, TOP, 128>(p, rows, stream);
 }
 
 }  // namespace lp
@@ -526,9 +526,13 @@ extern "C" int cpi_log_probs(const void* logits, int dtype, long stride, int row
   const long enough = 2l * sm_count();
   while (cluster < lp::kMaxCluster && (long)rows * cluster * 2 <= enough && vocab / (cluster * 2) >= 2048) cluster *= 2;
   lp::Params p{logits, stride, vocab, targets, n_targets, wide_targets, logprob, entropy, top_v, top_i, top, cluster};
-  const bool wide = rows * cluster <= enough;
-  if (dtype == kF32) return top ? lp::launch<float, true>(p, rows, wide, stream) : lp::launch<float, false>(p, rows, wide, stream);
-  if (dtype == kBF16) return top ? lp::launch<__nv_bfloat16, true>(p, rows, wide, stream) : lp::launch<__nv_bfloat16, false>(p, rows, wide, stream);
+  // Threads of a block: 512 where the blocks fill no more than the device at once (8 x 202,048 float32, 64 blocks: 10.6 us, with 256 12.2).
+  // More blocks than that hide each other's ends, which are many barriers long: 256 (1,000 x 151,643 bfloat16: 68 us, with 512 83, with 128
+  // 75), or 128 where rows are short and many (2,000 rows of 500 / 4,000 / 16,000 float32: 9.4 / 13.9 / 29 us, with 256 16.2 / 17.6 /
+  // 33; 600 of 16,000: 17.0 and 14.4).
+  const int threads = (long)rows * cluster <= enough ? 512 : vocab <= 16384 && rows >= 8 * sm_count() ? 128 : 256;
+  if (dtype == kF32) return top ? lp::launch<float, true>(p, rows, threads, stream) : lp::launch<float, false>(p, rows, threads, stream);
+  if (dtype == kBF16) return top ? lp::launch<__nv_bfloat16, true>(p, rows, threads, stream) : lp::launch<__nv_bfloat16, false>(p, rows, threads, stream);
   set_error("log_probs: unknown dtype code %d", dtype);
   return 1;
 }

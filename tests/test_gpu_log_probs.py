@@ -44,7 +44,7 @@ def compare(x, targets, top):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (1, 2, 0), (3, 5, 5), (2, 31, 20), (1, 500, 32), (7, 1001, 1), (1, 32000, 5), (5, 32003, 32),
-                                            (1, 202048, 20), (8, 202048, 20), (40, 65537, 7), (300, 4099, 3), (1000, 777, 0)])
+                                            (1, 202048, 20), (8, 202048, 20), (40, 65537, 7), (300, 4099, 3), (1000, 777, 0), (1300, 129, 32), (1300, 5001, 20), (1184, 16384, 1)])
 def test_random_rows(dtype, rows, vocab, top):
     g = torch.Generator(device=DEV).manual_seed(vocab + rows)
     x = (torch.randn(rows, vocab, generator=g, device=DEV) * 4).to(dtype)
