@@ -80,21 +80,25 @@ class Kv8Plan:
                 seen = min(seen, -(-(window_size + 256 + self.window[2]) // BLOCK) + 2)
             self.most_tiles = max(self.most_tiles, seen // 2 + 2)
         at = self.n_earlier
-        jobs = []
+        jobs = []                  # rows of eight numbers: slot, block, first new row, rows, earlier page, exact page, last page, last rows
         for i, (s, e) in enumerate(zip(starts, ends)):
             first, n_blocks = s // BLOCK, -(-e // BLOCK)
-            tables[1, i, first:n_blocks] = np.arange(at, at + n_blocks - first)
-            last_rows = e - (n_blocks - 1) * BLOCK
-            for b in range(first, n_blocks):
-                keeps_tail = b == first
-                jobs.append((slots[i], b, s - b * BLOCK if b == first else 0, min(BLOCK, e - b * BLOCK), tables[0, i, b], at + b - first,
-                             at + n_blocks - 1 - first if keeps_tail else -1, last_rows))
+            own = np.arange(first, n_blocks)
+            tables[1, i, first:n_blocks] = at + own - first
+            job = np.empty((len(own), 8), dtype=np.int32)
+            job[:, 0], job[:, 1], job[:, 2], job[:, 3] = slots[i], own, 0, np.minimum(BLOCK, e - own * BLOCK)
+            job[:, 4], job[:, 5], job[:, 6], job[:, 7] = tables[0, i, first:n_blocks], at + own - first, -1, e - (n_blocks - 1) * BLOCK
+            job[0, 2], job[0, 6] = s - first * BLOCK, at + n_blocks - 1 - first       # the first one reads the tail, then keeps it
+            jobs.append(job)
             at += n_blocks - first
         for i, s in enumerate(starts):
-            for b in np.flatnonzero(tables[0, i, :s // BLOCK] >= 0):
-                jobs.append((slots[i], b, 0, BLOCK, tables[0, i, b], -1, -1, 0))
+            earlier = np.flatnonzero(tables[0, i, :s // BLOCK] >= 0)
+            job = np.zeros((len(earlier), 8), dtype=np.int32)
+            job[:, 0], job[:, 1], job[:, 3], job[:, 4], job[:, 5:7] = slots[i], earlier, BLOCK, tables[0, i, earlier], -1
+            jobs.append(job)
+        jobs = np.concatenate(jobs)
         self.n_pages, self.n_jobs = at, len(jobs)
-        flat = np.concatenate([tables.ravel(), np.arange(n, dtype=np.int32), np.asarray(jobs, dtype=np.int32).ravel()])
+        flat = np.concatenate([tables.ravel(), np.arange(n, dtype=np.int32), jobs.ravel()])
         host = torch.from_numpy(flat)
         dev = torch.device(device)
         if dev.type == "cuda":
