@@ -233,9 +233,17 @@ __global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kern
     abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // Positions, slots and the page table are in place before the kernels in front of this one begin (see common.cuh): they are
-  // read under those kernels' ends, the cache and the queries after them.
+  __syncthreads();                                          // the barriers are ready
+  pdl_wait();
+  pdl_launch_dependents();                                  // (in this order: it reads cached rows, see common.cuh)
   const int G = p.n_heads / p.n_kv_heads;
+  const __nv_bfloat16* q = p.q + ((size_t)t * p.n_heads + (size_t)kvh * G) * D;
+  uint2 raw[HT][NC];                                        // asked for before the indices, which are a chain of four reads
+#pragma unroll
+  for (int h = 0; h < HT; ++h)
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      raw[h][c] = h * 8 + g < G ? *reinterpret_cast<const uint2*>(q + (size_t)(h * 8 + g) * D + c * 16 + 4 * j) : make_uint2(0u, 0u);
   int pos = p.token_pos[t];
   const int seq = p.token_seq[t];
   int slot = seq >= 0 && seq < p.n_seqs ? p.seq_slot[seq] : -1;
@@ -285,18 +293,8 @@ __global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kern
     }
   };
   take_ids(0);
-  __syncthreads();                                          // the barriers are ready
-  pdl_wait();
-  pdl_launch_dependents();                                  // (in this order: it reads cached rows, see common.cuh)
 #pragma unroll
   for (int y = 0; y < SLOTS; ++y) ask(y, y);
-  const __nv_bfloat16* q = p.q + ((size_t)t * p.n_heads + (size_t)kvh * G) * D;
-  uint2 raw[HT][NC];
-#pragma unroll
-  for (int h = 0; h < HT; ++h)
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-      raw[h][c] = h * 8 + g < G ? *reinterpret_cast<const uint2*>(q + (size_t)(h * 8 + g) * D + c * 16 + 4 * j) : make_uint2(0u, 0u);
 
   {
     // the own block: four warps of the last split take 16 of its positions each

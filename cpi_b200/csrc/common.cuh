@@ -73,7 +73,7 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
 // predecessor's tail.
 // Two things besides weights are read before the wait, by few kernels and under a condition each.  A step's index arrays
 // (positions, slots, page tables, runs of tokens) come from copies that end before the step's first kernel starts: read by
-// attention_decode, attention_decode_kv8, qkv_post_d128, qkv_conv_rotate and head_turn.  Cached pages, all but the one that holds the newest position:
+// attention_decode, qkv_post_d128, qkv_conv_rotate and head_turn.  Cached pages, all but the one that holds the newest position:
 // read by attention_decode.  Their rows come from earlier launches, each of which an attention kernel followed, and those that read
 // cached keys let their successors start only after their own wait, when the rows have been stored: whatever starts later
 // finds them.  So steps may follow one another without anything between them; but between a launch that stores several

@@ -1202,9 +1202,8 @@ def attention_decode_kv8(q, out, cache, page_table, token_seq, token_pos, seq_sl
     the tail's codes and scales are written to page page_table[slot, b].  `max_context`: no sequence is longer (it sizes the
     division of the keys over blocks of threads; any number is right, a good one is fast).  Windows, kept first positions,
     sink and soft cap as in `attention_decode`.  A token at a negative position is a padded row: its output is zero.  Tokens
-    of a call belong to different slots.  The index arrays and the page table are read before the kernels in front of this one
-    end: no kernel of this library may be writing them (copies and other kernels have ended by then).  An index outside
-    of the cache sets the error word (`device_error_flags`) and gives zeros; nothing is read or written for it."""
+    of a call belong to different slots.  An index outside of the cache sets the error word (`device_error_flags`) and gives
+    zeros; nothing is read or written for it."""
     what = "attention_decode_kv8"
     fmt, nkv, d, slots, at = _kv8(cache, what, n_heads)
     T, table = q.shape[0], page_table.shape

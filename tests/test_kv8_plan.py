@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import random
+import re
 
 import pytest
 import torch
@@ -10,6 +11,7 @@ import kv8_plain as P
 from cpi_b200.cache.kv8 import Kv8Cache, Kv8Plan, needed_blocks
 from cpi_b200.cache.manager import KVRequirement
 from cpi_b200.csrc import lib as K
+from test_kernel_order import KERNELS
 
 
 def draws(n):
@@ -146,3 +148,15 @@ def test_arguments_are_declared_as_the_library_has_them():
         args = re.search(r'extern "C" int ' + name + r"\(([^)]*)\)", sources).group(1).split(",")
         kinds = ["p" if "*" in a or "cudaStream_t" in a else "f" if "float " in a else "l" if "long " in a else "i" for a in args]
         assert "".join(kinds) == types, name
+
+
+@pytest.mark.parametrize("name", ["attention_decode_kv8.cu:attention_decode_kv8_kernel", "attention_prefill_kv8.cu:attention_prefill_kv8_kernel",
+                                  "kv8_stage.cu:kv8_stage_kernel", "log_probs.cu:log_probs_kernel",
+                                  "attention_decode_kv8.cu:attention_decode_kv8_combine", "attention_prefill_kv8.cu:attention_prefill_combine"])
+def test_kernels_wait_before_they_read_and_before_their_successors_start(name):
+    """Indices, codes, tails and logits may come from the kernel in front: nothing is read through a pointer before the wait, and
+    successors, whose predecessors have to have stored their rows, start after it."""
+    body = KERNELS[name]
+    before = body[:body.index("pdl_wait()")]
+    assert not re.search(r"\bp\.\w+\s*\[|\bpart_\w+\s*\[|tma_load|\bjob\s*\[|__ldcg|\*reinterpret_cast", before)
+    assert all(body.index("pdl_wait()") < m.start() for m in re.finditer(r"pdl_launch_dependents\(\)", body))
