@@ -138,6 +138,10 @@ def validate(a) -> None:
         bad("--no-repeat-ngram must be >= 0")
     if a.logprobs is not None and not 0 <= a.logprobs <= 32:
         bad("--logprobs must be in [0, 32]")
+    if a.interactive and (a.score or a.logprobs is not None):
+        bad("--score and --logprobs print scores, which --interactive's events do not have")
+    if a.score and (a.benchmark or a.dump_logits):
+        bad("--score runs by itself: without --benchmark and --dump-logits")
     if a.cache_dtype is not None and a.dtype in ("float32", "fp32"):
         bad("--cache-dtype goes with --dtype bfloat16")
     if a.benchmark_reps < 1 or a.benchmark_warmup < 0:

@@ -24,9 +24,9 @@ def score_sequence(engine, tokens: Sequence[int], top: int = 0) -> "K.LogProbs":
         raise ValueError("a sequence to score has two tokens or more: the first is given, the others are scored")
     n = len(tokens) - 1
     piece = max(1, min(engine.max_step_tokens, LOGIT_BYTES // (4 * engine.spec.vocab_size)))
-    targets = torch.tensor(tokens[1:], dtype=torch.int32, device=engine.device)
-    if int(min(tokens)) < 0 or int(max(tokens)) >= engine.spec.vocab_size:
+    if min(tokens) < 0 or max(tokens) >= engine.spec.vocab_size:
         raise ValueError(f"a token id lies outside the vocabulary of {engine.spec.vocab_size}")
+    targets = torch.tensor(tokens[1:], dtype=torch.int32, device=engine.device)
     slot = engine.acquire_slot()
     parts = []
     try:

@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import random
 import re
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -160,3 +161,20 @@ def test_kernels_wait_before_they_read_and_before_their_successors_start(name):
     before = body[:body.index("pdl_wait()")]
     assert not re.search(r"\bp\.\w+\s*\[|\bpart_\w+\s*\[|tma_load|\bjob\s*\[|__ldcg|\*reinterpret_cast", before)
     assert all(body.index("pdl_wait()") < m.start() for m in re.finditer(r"pdl_launch_dependents\(\)", body))
+
+
+@pytest.mark.parametrize("tokens", [[], [3], [1, 50], [1, -1], [1, 2 ** 31], [2 ** 40, 1]])
+def test_sequences_that_are_not_scored(tokens):
+    from cpi_b200.engine.score import score_sequence
+    engine = SimpleNamespace(spec=SimpleNamespace(vocab_size=50), max_step_tokens=8, device="cpu")
+    with pytest.raises(ValueError):
+        score_sequence(engine, tokens)
+
+
+@pytest.mark.parametrize("argv", [["--interactive", "--logprobs", "2"], ["--interactive", "--score"], ["--score", "--benchmark"],
+                                  ["--score", "--dump-logits", "x"], ["--logprobs", "33"], ["--logprobs", "-1"],
+                                  ["--cache-dtype", "int8", "--dtype", "float32"]])
+def test_options_of_the_command_line_that_do_not_go_together(argv, capsys):
+    from cpi_b200.cli import llama_infer as cli
+    assert cli.main(["m", *argv]) == 1
+    assert argv[0] in capsys.readouterr().err
