@@ -13,7 +13,8 @@
 // The axis of key tiles begins with the exact tiles of A (those that hold its own blocks), goes on with the earlier blocks' and ends
 // with the exact tiles of B: A meets a prefix of it and B a suffix.  A row's mask is that of the window cut at the start of its block,
 // from one side or the other.  Pages that a tile does not have are asked for beyond the tensor's end and arrive as zeros, rows behind
-// the newest position are zero already: nothing is overwritten in shared memory.  Per query tile that is one or two key tiles more
+// the newest position are zero already: nothing is overwritten in shared memory.  A masked weight is a zero in the product P V, so a
+// value that is not finite also reaches queries of its sequence that do not see it, in the same key tile.  Per query tile that is one or two key tiles more
 // than over a cache in bfloat16 (they hold the own blocks twice).
 //
 // Softmax: warps 0-3 own query tile A, warps 4-7 tile B; thread r of a group owns query row r and all 128 columns of a tile.  A row's

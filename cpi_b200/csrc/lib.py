@@ -1261,7 +1261,8 @@ def attention_prefill_kv8(q, out, k_pages, v_pages, plan, token_seq, token_pos, 
                           window_kind=WINDOW_FULL, window_size=0, keep_first=0, sink=None, softcap=0.0):
     """Attention of a step's tokens over the pages that `kv8_stage` has prepared: each query sees its own block of 64
     positions in the exact pages and earlier ones in the earlier pages.  q, out bfloat16 [T, n_heads * head_dim]; query
-    tiles as in `attention_prefill`; the window is the plan's."""
+    tiles as in `attention_prefill`; the window is the plan's.  Values are finite: one that is not makes NaN of outputs of its
+    own sequence that do not see it (a masked weight is a zero in a product); other sequences are not touched."""
     what = "attention_prefill_kv8"
     shape = k_pages.shape
     if len(shape) != 4 or shape[2] != 64 or shape[3] not in (64, 128):

@@ -438,6 +438,48 @@ def test_captured_and_replayed_beside_an_eager_call():
         rig.check(0, q.view(1, 8, 128), out.view(1, 8, 128), [3000])
 
 
+def test_a_sequence_that_is_not_finite_leaves_the_others_alone():
+    """Sequences of one step lie side by side in the packed tokens and in the step's pages; what one holds reaches no other."""
+    for fmt in ("int8", "e4m3"):
+        rig = Rig([90, 70, 200], fmt=fmt, nh=4, nkv=2, d=64, seed=31)
+        rig.k[1][3], rig.v[1][5], rig.v[1][69] = math.inf, math.nan, -math.inf
+        q, out, _ = rig.prompt([90, 70, 200])
+        assert out[1][69].isnan().any()
+        for i, n in ((0, 90), (2, 200)):
+            rig.check(i, q[i], out[i], list(range(n)))
+            rig.check_held(i)
+
+
+def test_prompts_at_once():
+    """Prompts of two caches on two streams, again and again: nothing is shared between the calls."""
+    news, done = [300, 65], []
+    rigs = [Rig(news, nh=4, nkv=2, seed=40 + i) for i in range(2)]
+    for rig in rigs:                                # what a prompt alone gives
+        q, out, _ = rig.prompt(news)
+        for i, n in enumerate(news):
+            rig.check(i, q[i], out[i], list(range(n)))
+        batch = rig.stager.stage(rig.slots, [0, 0], [[0] * m for m in news], [[]] * 2, torch.bfloat16)
+        plan = Kv8Plan([0, 0], news, rig.slots, device=DEV)
+        pages = [torch.zeros(plan.n_pages, 2, BLOCK, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+        at, row = plan.exact_table.long()[batch.token_seq.long(), (batch.token_pos // BLOCK).long()], (batch.token_pos % BLOCK).long()
+        for to, x in zip(pages, (rig.k, rig.v)):
+            to[at, :, row] = torch.cat(x)
+        done.append((rig, torch.cat(q).view(sum(news), -1), torch.cat(out).view(sum(news), -1), plan, batch, pages))
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(5):
+        for s, (rig, q, _, plan, batch, pages) in zip(streams, done):
+            with torch.cuda.stream(s):
+                out = torch.zeros_like(q)
+                K.kv8_stage(rig.cache, rig.table, plan, *pages)
+                K.attention_prefill_kv8(q, out, *pages, plan, batch.token_seq, batch.token_pos, batch.tile_tok0, batch.tile_rows, n_heads=4,
+                                        scale=128 ** -0.5)
+                outs.append(out)
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        assert torch.equal(out, done[i % 2][2])
+
+
 def test_same_results_twice():
     rig = Rig([2000, 77], nh=8, nkv=2, seed=25)
     for i, p in enumerate((1999, 76)):

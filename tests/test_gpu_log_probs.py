@@ -113,6 +113,13 @@ def test_targets_that_are_none():
     assert abs(float(got[0, 2] - want[0, 3])) < 1e-5 and abs(float(got[1, 1] - want[1, 99])) < 1e-5
 
 
+def test_targets_beyond_32_bits():
+    """Their low halves would name tokens of the vocabulary."""
+    x = torch.randn(2, 100, device=DEV)
+    got = K.log_probs(x, torch.tensor([[2 ** 32 + 5, 2 ** 40], [-2 ** 32 + 5, -2 ** 62]], device=DEV), top=0).logprob
+    assert got[0].isnan().all() and got[1].tolist() == [0.0, 0.0]
+
+
 def test_large_logits_and_peaks():
     x = torch.randn(4, 9001, device=DEV) * 1e4
     x[1] = x[1] * 1e-4 + 3e4
