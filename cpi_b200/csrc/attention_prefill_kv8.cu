@@ -18,23 +18,28 @@
 // than over a cache in bfloat16 (they hold the own blocks twice).
 //
 // Softmax: warps 0-3 own query tile A, warps 4-7 tile B; thread r of a group owns query row r and all 128 columns of a tile.  A row's
-// reference m is raised, and O rescaled in tensor memory, only when the row maximum has outgrown it by 2^40: P is bfloat16 and the
-// sums are float32, which have the same range of powers, so nothing is lost by numbers up to 2^40 (sums up to 2^57, outputs finite
-// for values up to 2^70), and it happens in a row's first tile and hardly ever again (keys and queries with a few large features,
-// 3,001 tokens of 40 heads: 190 us with 2^8, 171 with 2^40).  Tiles without a mask take one pass against the reference they have;
-// all others two small loops, the maximum and then the exponentials, whose P goes over columns of S that have been read: a block of
-// threads meets most of this code cold, and one pass for all cases was more than an instruction cache holds.  Columns that no row of
-// the warp sees are passed over.
+// reference m is its first tile's maximum, raised (and O rescaled in tensor memory) only when the row maximum has outgrown it by
+// 2^40: P is bfloat16 and the sums are float32, which have the same range of powers, so nothing is lost by numbers up to 2^40 (sums up
+// to 2^57, outputs finite for values up to 2^70), and it happens in a row's first tile and hardly ever again (keys and queries with a
+// few large features, 3,001 tokens of 40 heads: 190 us with 2^8, 171 with 2^40).  Tiles without a mask are taken into registers
+// whole, the maximum first, then P and the sum with two numbers to an instruction.  Masked tiles, and those that outgrow a reference,
+// go by 32 columns with the next ones on their way, against the reference they have; what has been stored of a tile's P is rescaled
+// too.  Columns that no row of the warp sees are passed over.
 //
-// Bound by the chain S -> softmax -> P V -> next S of each query tile: about 4,100 cycles for two tiles of 128 x 128, where the
-// products take 2,048 and the exponentials as many.  3,001 tokens of 40/8 heads of 128: 149 us (620 TFLOP/s; the tensor pipe
-// stands still half of the time).  What was tried beside it: two threads to a row, sixteen warps, either spill with 96 registers each (238
-// us) or read S twice (168); a quarter of the exponentials as polynomials 160; waiting for the next tiles after P instead of before
-// it 155; without the look that does not suspend (wait_soon) 157.
+// Bound by the chain S -> softmax -> P V -> next S of each query tile (about 3,600 cycles for two tiles of 128 x 128, where the products
+// take 2,048 and the exponentials as many) and by a block's start and end, which nothing hides (6,000 cycles from its first
+// instruction to its first S: indices, page numbers, loads; 3,000 at the end).  3,001 tokens of 40/8 heads of 128: 123 us (750 TFLOP/s).
+// The way there: 149 with one number to an instruction, masked and first tiles in two passes, and each thread writing its own row 16
+// bytes at a time (8,000 cycles a block); two numbers to an instruction and the maximum of three 146; rows written as whole lines
+// 135; masked tiles in one pass and first tiles, if nothing is masked, from registers 123.  What was tried beside it: two threads
+// to a row, sixteen warps, either spill with 96 registers each or read S twice; a quarter of the exponentials as polynomials; P
+// handed on in two halves (the issuing warp then waits for one tile's second half while the other's is ready); every tile by 32
+// columns (a vote each; 141): all slower.
 //
 // Few query tiles over many keys share their key tiles out among blocks of threads (n_splits), joined by a second kernel.
 // Every mbarrier wait is bounded; when one runs out the block sets *error_flag and leaves.
 #include "prefill_tc.cuh"
+#include "f32x2.cuh"
 #include "packed.cuh"
 #include <type_traits>
 
@@ -70,6 +75,27 @@ __device__ __forceinline__ bool wait_soon(uint64_t* bar, uint32_t parity, volati
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
   return ok != 0 || mbar_wait(bar, parity, abort_flag);
+}
+// The largest of three (a NaN is passed over).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The loads issued so far have landed in these registers (named, so that nothing reads them before).
+__device__ __forceinline__ void landed32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+        "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+        "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+        "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+      :: "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  tmem_ld16_issue(taddr, r);
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+        "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
 }
 template <int D, bool CAPPED>
 __global__ void __launch_bounds__(kThreads, 1) attention_prefill_kv8_kernel(const __grid_constant__ CUtensorMap map_q,
@@ -325,86 +351,147 @@ __global__ void __launch_bounds__(kThreads, 1) attention_prefill_kv8_kernel(cons
         return visible(qp, lo, keep, first) & (exact ? ~before : before);
       };
       bool stored = false;
-      if (!CAPPED && no_mask && j > 0) {
-        uint32_t w[BKV / 32][16], raw[BKV / 32][32];
-        const float nref = -m_ref;
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, ls4[4] = {0.f, 0.f, 0.f, 0.f};
+      if (!CAPPED && no_mask) {
+        uint32_t r[BKV / 32][32];
 #pragma unroll
-        for (int cc = 0; cc < BKV / 32; ++cc) tmem_ld32_issue(s_row + cc * 32, raw[cc]);
-        tmem_wait_ld();
+        for (int c = 0; c < BKV / 32; ++c) tmem_ld32_issue(s_row + c * 32, r[c]);
 #pragma unroll
-        for (int cc = 0; cc < BKV / 32; ++cc) {
-          float v[32];
+        for (int c = 0; c < BKV / 32; ++c) landed32(r[c]);
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float sv = __uint_as_float(raw[cc][e]);
-            mx4[e & 3] = fmaxf(mx4[e & 3], sv);
-            v[e] = exp2_fast(fmaf(sv, sc, nref));
-          }
+        for (int c = 0; c < BKV / 32; ++c)
 #pragma unroll
-          for (int e = 0; e < 32; ++e) ls4[e & 3] += v[e];
-#pragma unroll
-          for (int g = 0; g < 16; ++g) w[cc][g] = pack_bf16(v[2 * g], v[2 * g + 1]);
-        }
+          for (int g = 0; g < 16; ++g) mx4[g & 3] = max3(mx4[g & 3], __uint_as_float(r[c][2 * g]), __uint_as_float(r[c][2 * g + 1]));
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+        if (j == 0) m_ref = fmaxf(mx, m_ref);
         stored = !__any_sync(0xffffffffu, mx > m_ref + (m_ref < -1e29f ? 0.f : kWideSlack));
         if (stored) {
+          const uint64_t sc2 = pair(sc, sc), nref2 = pair(-m_ref, -m_ref);
+          uint64_t sum2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
-          for (int cc = 0; cc < BKV / 32; ++cc) tmem_st16_nowait(s_row + cc * 16, w[cc]);
-          l_run += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
+          for (int c = 0; c < BKV / 32; ++c) {
+            uint32_t w[16];
+#pragma unroll
+            for (int g = 0; g < 16; ++g) {
+              const float2 z = unpair(fma2(pair(__uint_as_float(r[c][2 * g]), __uint_as_float(r[c][2 * g + 1])), sc2, nref2));
+              const float e0 = exp2_fast(z.x), e1 = exp2_fast(z.y);
+              sum2[g & 1] = add2(sum2[g & 1], pair(e0, e1));
+              w[g] = pack_bf16(e0, e1);
+            }
+            tmem_st16_nowait(s_row + c * 16, w);
+          }
+          const float2 sum = unpair(add2(sum2[0], sum2[1]));
+          l_run += sum.x + sum.y;
         }
       }
       if (!stored) {
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < BKV; c += 32) {
-          const uint32_t in = no_mask ? 0xffffffffu : sees(key0 + c);
-          if (!__any_sync(0xffffffffu, in != 0)) continue;
-          float v[32], mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          tmem_ld32(s_row + c, v);
+        auto seen = [&](int c) { return no_mask ? 0xffffffffu : sees(key0 + c * 32); };      // of columns 32 c .. 32 c + 31 by this row
+        uint32_t some = 0, any = 0;                        // bit c: some row of the warp sees some of chunk c; columns that this row sees
 #pragma unroll
-          for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], (in >> e) & 1u ? v[e] : -INFINITY);
-          mx = fmaxf(mx, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
+        for (int c = 0; c < BKV / 32; ++c) {
+          const uint32_t in = seen(c);
+          any |= in;
+          some |= __any_sync(0xffffffffu, in != 0) ? 1u << c : 0u;
         }
-        mx = CAPPED && mx > -INFINITY ? tanh_fast(mx * cap_in) * sc : mx * sc;
-        const bool grow = mx > m_ref + (m_ref < -1e29f ? 0.f : kWideSlack);
-        if (j == 0) {
-          m_ref = fmaxf(mx, m_ref);
-        } else if (__any_sync(0xffffffffu, grow)) {
-          const float m_new = grow ? mx : m_ref, f = exp2f(m_ref - m_new);
-          // Every P V issued so far for this query tile has landed: the Q K^T whose S was waited for above was issued after the
-          // last of them, and its arrival covers everything issued before it.
+        if (__any_sync(0xffffffffu, m_ref < -1e29f && any)) {
+          // rows that have seen nothing so far (of their O and sum there is nothing to rescale)
+          float mx = -INFINITY;
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            float v[32];
-            tmem_ld32(o_row + c, v);
+          for (int c = 0; c < BKV / 32; ++c) {
+            if (!(some >> c & 1u)) continue;
+            const uint32_t in = seen(c);
+            uint32_t r[32];
+            tmem_ld32_issue(s_row + c * 32, r);
+            landed32(r);
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] *= f;
-            tmem_st32(o_row + c, v);
+            for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], (in >> e) & 1u ? __uint_as_float(r[e]) : -INFINITY);
+            mx = fmaxf(mx, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
           }
-          l_run *= f;
-          m_ref = m_new;
+          mx = CAPPED && mx > -INFINITY ? tanh_fast(mx * cap_in) * sc : mx * sc;
+          if (m_ref < -1e29f) m_ref = fmaxf(mx, m_ref);
         }
-        const float nref = -m_ref;
-#pragma unroll 1
-        for (int c = 0; c < BKV; c += 32) {
-          const uint32_t in = no_mask ? 0xffffffffu : sees(key0 + c);
-          uint32_t w[16] = {};
-          if (__any_sync(0xffffffffu, in != 0)) {
-            float v[32], ls4[4] = {0.f, 0.f, 0.f, 0.f};
-            tmem_ld32(s_row + c, v);
+        const uint64_t sc2 = pair(sc, sc);
+        uint64_t sum2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+        auto chunk = [&](int c, uint32_t (&r)[32]) {       // scores in r -> P, stored over columns of S that have been read
+          uint32_t w[16];
+          if (some >> c & 1u) {
+            if (CAPPED || !no_mask) {
+              const uint32_t in = seen(c);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              if (CAPPED) v[e] = tanh_fast(v[e] * cap_in);
-              v[e] = (in >> e) & 1u ? exp2_fast(fmaf(v[e], sc, nref)) : 0.f;
-              ls4[e & 3] += v[e];
+              for (int e = 0; e < 32; ++e) {
+                float v = __uint_as_float(r[e]);
+                if (CAPPED) v = tanh_fast(v * cap_in);
+                r[e] = (in >> e) & 1u ? __float_as_uint(v) : 0xff800000u;
+              }
             }
+            while (true) {
+              const uint64_t nref2 = pair(-m_ref, -m_ref);
+              uint64_t part[2] = {sum2[0], sum2[1]};
+              float mx2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int g = 0; g < 16; ++g) w[g] = pack_bf16(v[2 * g], v[2 * g + 1]);
-            l_run += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
+              for (int g = 0; g < 16; ++g) {
+                const float a = __uint_as_float(r[2 * g]), b = __uint_as_float(r[2 * g + 1]);
+                mx2[g & 1] = max3(mx2[g & 1], a, b);
+                const float2 z = unpair(fma2(pair(a, b), sc2, nref2));
+                const float e0 = exp2_fast(z.x), e1 = exp2_fast(z.y);
+                part[g & 1] = add2(part[g & 1], pair(e0, e1));
+                w[g] = pack_bf16(e0, e1);
+              }
+              const float mx = fmaxf(mx2[0], mx2[1]) * sc;
+              const bool grow = mx > m_ref + kWideSlack;
+              if (!__any_sync(0xffffffffu, grow)) {
+                sum2[0] = part[0];
+                sum2[1] = part[1];
+                break;
+              }
+              // A row's maximum has outgrown its reference, which is raised by a whole number: the factor is a power of two, so P that
+              // has been rounded is not rounded again.  Every P V issued so far for this query tile has landed: the Q K^T whose S
+              // was waited for above was issued after the last of them, and its arrival covers everything issued before it.
+              const float m_new = grow ? fmaxf(m_ref + ceilf(mx - m_ref), mx) : m_ref, f = exp2f(m_ref - m_new);
+              tmem_wait_st();
+#pragma unroll 1
+              for (int at = 0; at < D; at += 16) {
+                uint32_t v[16];
+                tmem_ld16(o_row + at, v);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                tmem_st16_nowait(o_row + at, v);
+              }
+#pragma unroll 1
+              for (int at = 0; at < c; ++at) {              // this tile's P so far
+                uint32_t v[16];
+                tmem_ld16(s_row + at * 16, v);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = pack_bf16(__uint_as_float(v[e] << 16) * f, __uint_as_float(v[e] & 0xffff0000u) * f);
+                tmem_st16_nowait(s_row + at * 16, v);
+              }
+              l_run *= f;
+              const float2 s0 = unpair(sum2[0]), s1 = unpair(sum2[1]);
+              sum2[0] = pair(s0.x * f, s0.y * f);
+              sum2[1] = pair(s1.x * f, s1.y * f);
+              m_ref = m_new;
+            }
+          } else {
+#pragma unroll
+            for (int g = 0; g < 16; ++g) w[g] = 0;
           }
-          tmem_st16_nowait(s_row + (c >> 1), w);
+          tmem_st16_nowait(s_row + c * 16, w);
+        };
+        uint32_t ra[32], rb[32];
+        tmem_ld32_issue(s_row, ra);
+        landed32(ra);
+#pragma unroll 1
+        for (int c = 0; c < BKV / 32; c += 2) {
+          tmem_ld32_issue(s_row + (c + 1) * 32, rb);
+          chunk(c, ra);
+          landed32(rb);
+          if (c + 2 < BKV / 32) tmem_ld32_issue(s_row + (c + 2) * 32, ra);
+          chunk(c + 1, rb);
+          if (c + 2 < BKV / 32) landed32(ra);
         }
+        const float2 sum = unpair(add2(sum2[0], sum2[1]));
+        l_run += sum.x + sum.y;
       }
       tmem_wait_st();
       fence_before_sync();
@@ -421,33 +508,51 @@ __global__ void __launch_bounds__(kThreads, 1) attention_prefill_kv8_kernel(cons
     ok = __all_sync(0xffffffffu, ok && mbar_wait(&o_done[x], 0, abort_flag));
     fence_after_sync();
     if (ok) {
+      // A thread has a row, a line of 128 bytes at a time; through shared memory (that of the queries, which are done with) the lines
+      // go out whole: 8 lanes to each.
+      uint8_t* mine = q_s + warp * 4096;
+      const size_t row0 = (size_t)(tok0 + x * BQ + (warp & 3) * 32) * p.n_heads + head;
+      const int n_rows = rows_x[x] - (warp & 3) * 32;     // of this warp (may be none)
+      // a sink adds 2^(sink log2 e - reference) to the row's sum and nothing to O; the exponent is capped so that a
+      // sink far above every score gives a huge finite sum
+      if (p.sink && p.n_splits == 1) l_run += exp2f(fminf(p.sink[head] * 1.4426950408889634f - m_ref, 120.f));
+      const float inv = 1.0f / fmaxf(l_run, 1e-20f);
+      auto put = [&](int chunk, uint4 v) { *reinterpret_cast<uint4*>(mine + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = v; };
+      auto lines = [&](uint8_t* to, size_t stride) {      // the warp's 32 lines to memory, `stride` bytes apart
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + (lane >> 3), chunk = lane & 7;
+          const uint4 v = *reinterpret_cast<const uint4*>(mine + r * 128 + ((chunk ^ (r & 7)) << 4));
+          if (r < n_rows) *reinterpret_cast<uint4*>(to + r * stride + chunk * 16) = v;
+        }
+        __syncwarp();
+      };
       if (p.n_splits > 1) {
-        float* dst = p.part_o + (at * p.n_splits + blockIdx.z) * D;
+        uint8_t* to = reinterpret_cast<uint8_t*>(p.part_o + (row0 * p.n_splits + blockIdx.z) * D);
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           float v[32];
           tmem_ld32(o_row + c, v);
-          if (live) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(dst + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-          }
+          for (int e = 0; e < 8; ++e)
+            put(e, make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3])));
+          lines(to + c * 4, (size_t)p.n_heads * p.n_splits * D * 4);
         }
       } else {
-        // a sink adds 2^(sink log2 e - reference) to the row's sum and nothing to O; the exponent is capped so that a
-        // sink far above every score gives a huge finite sum
-        if (p.sink) l_run += exp2f(fminf(p.sink[head] * 1.4426950408889634f - m_ref, 120.f));
-        const float inv = 1.0f / fmaxf(l_run, 1e-20f);
-        __nv_bfloat16* dst = p.out + at * D;
+        uint8_t* to = reinterpret_cast<uint8_t*>(p.out + row0 * D);
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          float v[32];
-          tmem_ld32(o_row + c, v);
-          if (live) {
+        for (int c = 0; c < D; c += 64) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(pack_bf16(v[e] * inv, v[e + 1] * inv), pack_bf16(v[e + 2] * inv, v[e + 3] * inv),
-                                                                  pack_bf16(v[e + 4] * inv, v[e + 5] * inv), pack_bf16(v[e + 6] * inv, v[e + 7] * inv));
+          for (int half = 0; half < 2; ++half) {
+            float v[32];
+            tmem_ld32(o_row + c + half * 32, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              put(half * 4 + e, make_uint4(pack_bf16(v[8 * e] * inv, v[8 * e + 1] * inv), pack_bf16(v[8 * e + 2] * inv, v[8 * e + 3] * inv),
+                                           pack_bf16(v[8 * e + 4] * inv, v[8 * e + 5] * inv), pack_bf16(v[8 * e + 6] * inv, v[8 * e + 7] * inv)));
           }
+          lines(to + c * 2, (size_t)p.n_heads * D * 2);
         }
       }
     }

@@ -20,6 +20,7 @@
 // probabilities -inf, entropy 0.  A row that holds NaN or +inf: log probabilities and entropy are NaN; NaN is never among the
 // best.  A target below zero stands for none (0 is returned), one beyond the vocabulary gives NaN.
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "packed.cuh"
 
 namespace cpi {
@@ -43,33 +44,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {          // the lar
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
-// Two float32 operations in one instruction.
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t a) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 struct Sums { float m, z, s; };           // largest x, sum 2^d, sum 2^d d with d = (x - m) log2 e
 __device__ __forceinline__ Sums merged(Sums a, Sums b) {
   Sums t;

@@ -370,6 +370,30 @@ def test_prompt_sink_and_cap(softcap):
     rig.check(0, q[0][some], out[0][some], some, sink=sink, softcap=softcap)
 
 
+@pytest.mark.parametrize("d,nkv", [(64, 1), (128, 2)])
+@pytest.mark.parametrize("how", [dict(), dict(window="sliding", size=300, keep=3), dict(softcap=500.0)])
+def test_scores_that_rise(d, nkv, how):
+    """Scores that go up by more than 2^40 in weight again and again, at the first and last columns of tiles and of their parts,
+    inside and outside of masked tiles: whatever was added up before is worth nothing then, and what follows is."""
+    n, done = 700, 90
+    rig = Rig([n], nh=2, nkv=nkv, d=d, seed=50)
+    u = (torch.randint(0, 2, (d,), generator=rig.g, device=DEV) * 2 - 1).float()
+    level = torch.randn(n, generator=rig.g, device=DEV)
+    jumps = [0, 3, 31, 32, 33, 63, 64, 95, 127, 128, 129, 200, 255, 256, 300, 383, 400, 511, 512, 600, 650, 690]
+    for i, at in enumerate(jumps):
+        level[at] = 38.0 * (i + 1)                  # (38 log2 e = 55; up to 836, what the tolerance covers)
+        if at + 1 not in jumps:
+            level[at + 1] = level[at] - 1.0
+    rig.k[0] = (level[:, None, None] * u * d ** -0.5 + 0.1 * torch.randn(n, nkv, d, generator=rig.g, device=DEV)).bfloat16()
+    rig.rows = lambda *shape: u.bfloat16().expand(*shape).contiguous()
+    rig.load(0, done)
+    q, out, _ = rig.prompt([n - done], **how)
+    rig.check(0, q[0], out[0], list(range(done, n)), **how)
+    rig.done = [0]
+    q, out, _ = rig.prompt([n], **how)
+    rig.check(0, q[0], out[0], list(range(n)), **how)
+
+
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_cuts_do_not_matter(fmt):
     """A sequence in one step, in pieces and token by token: the same cache bit for bit, the same outputs as the definition."""
