@@ -14,8 +14,8 @@
 // with the exact tiles of B: A meets a prefix of it and B a suffix.  A row's mask is that of the window cut at the start of its block,
 // from one side or the other.  Pages that a tile does not have are asked for beyond the tensor's end and arrive as zeros, rows behind
 // the newest position are zero already: nothing is overwritten in shared memory.  A masked weight is a zero in the product P V, so a
-// value that is not finite also reaches queries of its sequence that do not see it, in the same key tile.  Per query tile that is one or two key tiles more
-// than over a cache in bfloat16 (they hold the own blocks twice).
+// value that is not finite also reaches queries of its sequence that do not see it, in the same key tile.  Per query tile that is one or
+// two key tiles more than over a cache in bfloat16 (they hold the own blocks twice).
 //
 // Softmax: warps 0-3 own query tile A, warps 4-7 tile B; thread r of a group owns query row r and all 128 columns of a tile.  A row's
 // reference m is its first tile's maximum, raised (and O rescaled in tensor memory) only when the row maximum has outgrown it by
@@ -32,9 +32,12 @@
 // The way there: 149 with one number to an instruction, masked and first tiles in two passes, and each thread writing its own row 16
 // bytes at a time (8,000 cycles a block); two numbers to an instruction and the maximum of three 146; rows written as whole lines
 // 135; masked tiles in one pass and first tiles, if nothing is masked, from registers 123.  What was tried beside it: two threads
-// to a row, sixteen warps, either spill with 96 registers each or read S twice; a quarter of the exponentials as polynomials; P
+// to a row, sixteen warps, either spill with 96 registers each or read S twice; P
 // handed on in two halves (the issuing warp then waits for one tile's second half while the other's is ready); every tile by 32
-// columns (a vote each; 141): all slower.
+// columns (a vote each; 141); one S for both query tiles, read into registers at once, with the score products two steps ahead (145:
+// the issuing warp's waits, 200 cycles each behind the exponentials of the warps beside it, leave the pipe idle); 224 registers for
+// the softmax warps (126): all slower.  A quarter of the exponentials as cubics on the multipliers takes 2% off and is not taken: it is
+// 7e-5 off and what is not finite would need a path of its own.
 //
 // Few query tiles over many keys share their key tiles out among blocks of threads (n_splits), joined by a second kernel.
 // Every mbarrier wait is bounded; when one runs out the block sets *error_flag and leaves.
@@ -144,6 +147,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_prefill_kv8_kernel(cons
     rows = min(max(rows, 1), min(kTileRows, p.n_tokens - tok0));
     if (!good && tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
   }
+  if (warp == kSoftmaxWarps && lane == 0) {               // the queries of both tiles, under the reads of what else there is to know
+    mbar_expect_tx(&q_full, Q_BYTES * (rows > BQ ? 2 : 1));
+    for (int x = 0; x < (rows > BQ ? 2 : 1); ++x)
+      for (int h = 0; h < HALVES; ++h)
+        tma_load_2d(q_s + x * Q_BYTES + h * HALF_BYTES, &map_q, &q_full, head * D + h * 64, tok0 + x * BQ);
+  }
   int seq = p.token_seq[tok0];
   // the tile's rows are consecutive positions of one sequence; rows 0-127 are query tile A, the rest tile B
   int pos_first = p.token_pos[tok0];
@@ -198,11 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_prefill_kv8_kernel(cons
 
   if (warp == kSoftmaxWarps) {
     if (lane == 0) {
-      // ---- TMA producer: Q of both tiles, then K(kt0), V(kt0), K(kt0 + 1), ... through the ring ----
-      mbar_expect_tx(&q_full, Q_BYTES * (has_b ? 2 : 1));
-      for (int x = 0; x < (has_b ? 2 : 1); ++x)
-        for (int h = 0; h < HALVES; ++h)
-          tma_load_2d(q_s + x * Q_BYTES + h * HALF_BYTES, &map_q, &q_full, head * D + h * 64, tok0 + x * BQ);
+      // ---- TMA producer: K(kt0), V(kt0), K(kt0 + 1), ... through the ring ----
       int n = 0;                                         // item of the ring: 2 (kt - kt0) for keys, + 1 for values
       for (int kt = kt0; kt < kt1 && ok; ++kt) {
         const int blk0 = key_tile(kt) * (BKV / PAGE);
