@@ -28,7 +28,7 @@
 //
 // Bound by the chain S -> softmax -> P V -> next S of each query tile (about 3,600 cycles for two tiles of 128 x 128, where the products
 // take 2,048 and the exponentials as many) and by a block's start and end, which nothing hides (6,000 cycles from its first
-// instruction to its first S: indices, page numbers, loads; 3,000 at the end).  3,001 tokens of 40/8 heads of 128: 123 us (750 TFLOP/s).
+// instruction to its first S: indices, page numbers, loads; 3,000 at the end).  3,001 tokens of 40/8 heads of 128: 122 us (757 TFLOP/s).
 // The way there: 149 with one number to an instruction, masked and first tiles in two passes, and each thread writing its own row 16
 // bytes at a time (8,000 cycles a block); two numbers to an instruction and the maximum of three 146; rows written as whole lines
 // 135; masked tiles in one pass and first tiles, if nothing is masked, from registers 123.  What was tried beside it: two threads
