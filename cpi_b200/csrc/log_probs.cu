@@ -95,6 +95,7 @@ struct Shared {
   Sums part[kMaxWarps];
   int n_list, n_short;
   __align__(16) int lane_max[32];         // the largest that threads of each lane number have met (see ordered())
+  __align__(16) int snapshot[kMaxWarps][32];      // of these, each warp's own (see bound_of())
   __align__(16) uint64_t list[kList];     // (when it has run over: every warp's best)
   __align__(16) uint64_t shorter[kShort];
   uint64_t top[kMaxTop];                  // the sorted best, 0 behind the last
@@ -124,16 +125,22 @@ __device__ __forceinline__ void put_key(uint32_t at, uint64_t v) { asm volatile(
 // A bound for the top-th best of what the block has met: of the 32 maxima over the threads of each lane number the top-th
 // largest.  Whole warps call it, with their running maxima; `together`: all of the block's, so that everyone's count.  (What some
 // of the threads have met gives a bound all the same, if a lower one, and maxima only grow: no need to wait for the others.)
+// The others raise the maxima meanwhile, so they are read once, into this warp's snapshot, and both the ranks and the result are
+// the snapshot's: 32 different numbers that have been met, of which `top` are not below the result.  (Read a second time for the
+// ranks, a maximum that has grown in between would count against its own older number, and the bound would come out too high.)
 __device__ __forceinline__ float bound_of(Shared& sh, float own, int top, bool together) {
   const int lane = threadIdx.x & 31;
   const int mine = ordered(own);
   if (mine > *reinterpret_cast<volatile int*>(&sh.lane_max[lane])) atomicMax(&sh.lane_max[lane], mine);
   if (together) __syncthreads(); else __syncwarp();
   const int v = *reinterpret_cast<volatile int*>(&sh.lane_max[lane]);
+  int* snapshot = sh.snapshot[threadIdx.x >> 5];
+  snapshot[lane] = v;
+  __syncwarp();
   int before = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int4 o = reinterpret_cast<const int4*>(sh.lane_max)[i];
+    const int4 o = reinterpret_cast<const int4*>(snapshot)[i];
     before += (o.x > v) + (o.y > v) + (o.z > v) + (o.w > v);
   }
   // the lanes with fewer than `top` before them; the least of their numbers is the top-th largest
