@@ -29,7 +29,9 @@ namespace lp {
 constexpr int UNROLL = 4, kMaxTop = 32, kMaxWarps = 16;
 constexpr int kList = 1024, kShort = 256; // keys kept beside the sums, and those of them that are sorted
 constexpr int kMaxCluster = 8;
-constexpr float kFloor = -1e38f;          // references begin here: what is below is as good as -inf unless a row has nothing else
+// References begin here, at a number of both types: what is below is as good as -inf unless a row has nothing else.  (As
+// bfloat16 numbers are coarser, one that they would round could lie above a thread's reference, and its exponential overflow.)
+constexpr float kFloor = -0x1p126f;
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kNone = 0x7fffffff;
@@ -44,14 +46,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {          // the lar
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
+// The exponent that a share's sums are scaled by, towards a larger reference: 0 for all that is 2^-200 or less, so that it stays
+// finite where the distance is beyond float32.  Every product of it is formed: zero times NaN keeps a NaN that a share has met.
+__device__ __forceinline__ float distance(float m, float top) { return fmaxf((m - top) * kLog2e, -200.f); }
 struct Sums { float m, z, s; };           // largest x, sum 2^d, sum 2^d d with d = (x - m) log2 e
 __device__ __forceinline__ Sums merged(Sums a, Sums b) {
   Sums t;
   t.m = fmaxf(a.m, b.m);
-  const float da = (a.m - t.m) * kLog2e, db = (b.m - t.m) * kLog2e, fa = ex2(da), fb = ex2(db);
-  // (a factor of zero drops its side: the distance may be beyond float32)
-  t.z = (fa > 0.f ? fa * a.z : 0.f) + (fb > 0.f ? fb * b.z : 0.f);
-  t.s = (fa > 0.f ? fa * fmaf(a.z, da, a.s) : 0.f) + (fb > 0.f ? fb * fmaf(b.z, db, b.s) : 0.f);
+  const float da = distance(a.m, t.m), db = distance(b.m, t.m), fa = ex2(da), fb = ex2(db);
+  // (products rounded before they are added: the same z in both lanes of a pair, so in all lanes of a warp)
+  t.z = __fadd_rn(__fmul_rn(fa, a.z), __fmul_rn(fb, b.z));
+  t.s = __fadd_rn(__fmul_rn(fa, fmaf(a.z, da, a.s)), __fmul_rn(fb, fmaf(b.z, db, b.s)));
   return t;
 }
 __device__ __forceinline__ Sums shifted(const Sums& a, int o) {
@@ -297,10 +302,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) log_probs_kernel(Params p) {
   }
   auto raise = [&](float top) {
     if (top > m) {
-      const float d = (m - top) * kLog2e, f = ex2(d);
-      const float2 z = unpair(z2), s = unpair(s2);
-      s2 = f > 0.f ? pair(f * fmaf(z.x, d, s.x), f * fmaf(z.y, d, s.y)) : pair(0.f, 0.f);
-      z2 = f > 0.f ? pair(f * z.x, f * z.y) : pair(0.f, 0.f);
+      const float d = distance(m, top), f = ex2(d);
+      s2 = mul2(fma2(z2, pair(d, d), s2), pair(f, f));
+      z2 = mul2(z2, pair(f, f));
       m = top;
     }
   };
@@ -418,7 +422,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) log_probs_kernel(Params p) {
   }
   bool empty = false;
   if (a.m <= kFloor) {
-    // nothing above -1e38 (masks of the type's lowest value, or of -inf): once more, against the true maximum
+    // nothing above kFloor (masks of the type's lowest value, or of -inf): once more, against the true maximum
     float top = -INFINITY;
     for (int i = tid; i < p.vocab; i += NT) top = fmaxf(top, to_f32(row[i]));
     top = block_max(top, sh.scratch);

@@ -2,6 +2,8 @@
 arithmetic."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -25,3 +27,42 @@ def test_the_best_of_rows_of_many_batches(rows, vocab, top, dtype):
         got = K.log_probs(x, targets, top=top)
         assert torch.equal(got.top_ids, ids)
         assert torch.equal(got.top_logprobs[:, -1], got.logprob[:, 0])
+
+
+def all_nan(got, r):
+    return bool(got.logprob[r].isnan().all() and got.entropy[r].isnan() and got.top_logprobs[r].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab,cover", [(33, 0), (3001, 0), (3001, 900), (40003, 5000), (151643, 0), (151643, 20000), (202048, 30000)])
+def test_a_nan_anywhere_in_a_row(vocab, cover, dtype):
+    """At the ends of rows that begin and end beside 16 bytes, in the middle, in any block's share, alone or among masked numbers
+    (`cover` of them to either side): the row's probabilities are NaN, the best tokens those of its numbers."""
+    places = [0, 1, vocab // 9, vocab // 3, vocab // 2 + 1, vocab - 1000 if vocab > 2000 else 5, vocab - 2, vocab - 1]
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    x = (torch.randn(len(places) + 1, vocab, generator=g, device=DEV) * 3).to(dtype)
+    for r, at in enumerate(places):
+        if cover:
+            x[r, max(0, at - cover):at + cover] = -math.inf
+        x[r, at] = math.nan
+    targets = torch.full((len(places) + 1, 2), vocab // 2, dtype=torch.int32, device=DEV)
+    got = K.log_probs(x, targets, top=4)
+    ids = torch.sort(x.nan_to_num(-math.inf, neginf=-math.inf), dim=-1, descending=True, stable=True).indices[:, :4].int()
+    assert torch.equal(got.top_ids, ids)
+    for r, at in enumerate(places):
+        assert all_nan(got, r), f"NaN at {at}"
+    assert got.logprob[-1].isfinite().all() and got.entropy[-1].isfinite() and got.top_logprobs[-1].isfinite().all()
+    bare = K.log_probs(x, targets)
+    assert bare.logprob[:-1].isnan().all() and bare.entropy[:-1].isnan().all() and bare.logprob[-1].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_short_rows_with_nan_and_infinities(dtype):
+    nan, inf = math.nan, math.inf
+    x = torch.tensor([[nan, nan, 1.0], [1.0, nan, -inf], [-inf, -inf, nan], [inf, 1.0, inf], [inf, -inf, 2.0], [nan, inf, -inf], [0.0, 0.0, -inf]],
+                     device=DEV).to(dtype)
+    got = K.log_probs(x, torch.zeros(7, dtype=torch.int32, device=DEV), top=3)
+    for r in range(6):
+        assert all_nan(got, r), f"row {r}"
+    assert got.top_ids.tolist() == [[2, -1, -1], [0, 2, -1], [0, 1, -1], [0, 2, 1], [0, 2, 1], [1, 2, -1], [0, 1, 2]]
+    assert abs(float(got.entropy[6]) - math.log(2)) < 1e-6 and abs(float(got.logprob[6]) + math.log(2)) < 1e-6
