@@ -421,8 +421,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) log_probs_kernel(Params p) {
     a = sh.sums[0];
   }
   bool empty = false;
-  if (a.m <= kFloor) {
-    // nothing above kFloor (masks of the type's lowest value, or of -inf): once more, against the true maximum
+  if (!(a.m > kFloor && a.m < -kFloor)) {
+    // Nothing above kFloor (masks of the type's lowest value, or of -inf), or a largest number from which kFloor is further than
+    // float32 goes (zero times that distance is NaN): once more, against the true maximum and the numbers as they are.
     float top = -INFINITY;
     for (int i = tid; i < p.vocab; i += NT) top = fmaxf(top, to_f32(row[i]));
     top = block_max(top, sh.scratch);

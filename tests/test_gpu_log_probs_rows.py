@@ -66,3 +66,26 @@ def test_short_rows_with_nan_and_infinities(dtype):
         assert all_nan(got, r), f"row {r}"
     assert got.top_ids.tolist() == [[2, -1, -1], [0, 2, -1], [0, 1, -1], [0, 2, 1], [0, 2, 1], [1, 2, -1], [0, 1, 2]]
     assert abs(float(got.entropy[6]) - math.log(2)) < 1e-6 and abs(float(got.logprob[6]) + math.log(2)) < 1e-6
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [5, 2999, 70001])
+@pytest.mark.parametrize("big", [0.9e38, 1.1e38, 1.5e38, 3e38])
+def test_numbers_near_the_types_largest(big, vocab, dtype):
+    """Distances beyond float32 are as good as infinite: nothing but the largest counts."""
+    x = torch.full((5, vocab), -math.inf, device=DEV)
+    x[0, 3] = big
+    x[1, 3], x[1, vocab - 1] = big, big
+    x[2, :], x[2, 3] = -big, big
+    x[3, :], x[3, 3], x[3, 4] = 0.0, big, -math.inf
+    x[4, :], x[4, 3] = -3e38, -big
+    x = x.to(dtype)
+    got = K.log_probs(x, torch.tensor([[3, 0]] * 5, dtype=torch.int32, device=DEV), top=2)
+    ties = [1, 2, 1, 1, 1 if big < 3e38 else vocab]
+    for r, n in enumerate(ties):
+        assert abs(float(got.entropy[r]) - math.log(n)) < 1e-5, f"row {r}"
+        assert abs(float(got.logprob[r, 0]) + math.log(n)) < 1e-5, f"row {r}"
+    want = torch.log_softmax(x.double(), -1)[:, 0]
+    for r in range(4):                   # (a distance of more than float32's largest is -inf)
+        w = float(want[r])
+        assert float(got.logprob[r, 1]) == (-math.inf if w < -3.4028235e38 else pytest.approx(w, rel=1e-6))
