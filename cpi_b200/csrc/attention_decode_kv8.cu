@@ -15,10 +15,11 @@
 //                     M, odd ones the lower.  P^T comes out of S^T's registers by movmatrix.
 // What a warp does for a tile is one long chain of dependent steps, so the count of warps decides: 64 sequences of up to 16,384
 // positions (40/8 heads of 128, e4m3) took 204 us with eight warps an SM at a page each (3,400 cycles a page, the data long there).
-// The queries are float16 too, each head's divided by a power of two (11 bits of significand hold bfloat16's 8 exactly; what is
-// 2^-22 below a head's largest element loses bits).  Scales act on scores in float32; the value scale 2^e enters the exponent: a
-// probability is p = 2^(s + e - m) with m the maximum of s + e, and the sum takes p 2^-e.  So blocks of any scale share one
-// accumulator, at no operation per output.
+// The queries are float16 too, each head's divided by a power of two that brings its largest element to 2^14 (11 bits of
+// significand hold bfloat16's 8 exactly; float16's smallest step is 2^-24, so an element loses bits only from 2^-31 of the
+// largest on; products stay below 2^24, far from float32's ends).  Scales act on scores in float32; the value scale 2^e enters
+// the exponent: a probability is p = 2^(s + e - m) with m the maximum of s + e, and the sum takes p 2^-e.  So blocks of any scale
+// share one accumulator, at no operation per output.
 // p is rounded to float16 (11 bits) against a reference m that is raised when s + e has outgrown it by 2^8, so the largest p lies
 // between 2^6 and 2^14: what is 2^-20 of the largest still has all its bits, smaller terms are off by 2^-31 of the largest at most.
 // (bfloat16 would keep 8 bits of all of them, but codes cost twice as many operations to become bfloat16.)  Sums, maxima and
@@ -319,8 +320,8 @@ __global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kern
       for (int c = 0; c < NC; ++c) top = max(top, kv8::top_of(make_uint4(raw[h][c].x, raw[h][c].y, 0u, 0u)));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // the largest element lies in [1, 2) after the division (a subnormal top: as it is, times 2^120)
-      const int e = max(-120, min(120, (int)(top >> 7) - 127));
+      // the largest element lies in [2^14, 2^15) after the division (below 2^-106: as it is, times 2^120)
+      const int e = max(-120, (int)(top >> 7) - 127 - 14);
       const float inv = kv8::power_of_two(-e);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
