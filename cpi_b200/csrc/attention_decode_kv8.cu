@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kern
   int slot = seq >= 0 && seq < p.n_seqs ? p.seq_slot[seq] : -1;
   // a position below zero is a padded row: it sees nothing and its output is zero
   if (pos >= 0 && (slot < 0 || slot >= p.n_slots || pos / PAGE >= p.max_blocks)) {
-    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, kIndexOutside);
     pos = -1;
   }
   const int lo = pos < 0 ? 0 : window_low(p.window_kind, p.window_size, pos);
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kern
     ids = x + lane < mine ? table[block_at(x + lane)] : 0;
     if (ids < 0 || ids >= total_pages) {                    // (beyond the map's last row: zeros arrive)
       ids = total_pages;
-      if (p.error_flag) atomicExch(p.error_flag, 3);
+      if (p.error_flag) atomicExch(p.error_flag, kIndexOutside);
     }
   };
   auto ask = [&](int y, int at) {                           // tile y into slot `at` (all lanes call it)
@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(Shape<D, HT>::NT, 2) attention_decode_kv8_kern
       const size_t to = (size_t)page * p.n_kv_heads + kvh;
       hold_tail<D, FMT, NT>(p.k_tail + tail, p.v_tail + tail, p.k + to * (PAGE * D), p.v + to * (PAGE * D), p.k_scale_w + to, p.v_scale_w + to, top_s);
     } else if (tid == 0 && p.error_flag) {
-      atomicExch(p.error_flag, 3);
+      atomicExch(p.error_flag, kIndexOutside);
     }
   }
   if (*aborted) {

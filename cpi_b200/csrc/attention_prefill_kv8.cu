@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_prefill_kv8_kernel(cons
     const bool good = tok0 >= 0 && tok0 < p.n_tokens && rows >= 1 && rows <= kTileRows && rows <= p.n_tokens - tok0;
     tok0 = min(max(tok0, 0), p.n_tokens - 1);
     rows = min(max(rows, 1), min(kTileRows, p.n_tokens - tok0));
-    if (!good && tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+    if (!good && tid == 0 && p.error_flag) atomicExch(p.error_flag, kIndexOutside);
   }
   if (warp == kSoftmaxWarps && lane == 0) {               // the queries of both tiles, under the reads of what else there is to know
     mbar_expect_tx(&q_full, Q_BYTES * (rows > BQ ? 2 : 1));
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_prefill_kv8_kernel(cons
   if (seq < 0 || seq >= p.n_seqs || pos_first < 0 || pos_first > p.width * PAGE - rows) {
     seq = 0;
     pos_first = 0;
-    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, kIndexOutside);
   }
   const int pos_last = pos_first + rows - 1;
   const int rows_x[2] = {min(rows, BQ), max(rows - BQ, 0)};

@@ -65,6 +65,10 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
   return r;
 }
 
+// What a kernel writes into the error word (device_error_flags in lib.py) when an index of a step lies outside of what it
+// belongs to.  Every other number there is a wait that ran out: 1, 2, 4, 5, by kind of kernel.
+constexpr int kIndexOutside = 3;
+
 // Programmatic dependent launch: a kernel launched with launch_pdl may start while the kernel before it in the stream is
 // still running.  Every such kernel calls pdl_wait() before it first reads or writes global memory that another kernel of
 // the stream produces or reads; pdl_wait() returns once the preceding kernel has finished and its writes are visible.

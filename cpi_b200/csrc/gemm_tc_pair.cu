@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(128) gemm_tc_pair_kernel(const __grid_constant
     direct<MODE, TO>(p, lane_addr, ACC == 2 ? lane_addr + BN : 0u, n, t0, n_valid_t, n_cols);
   }
   if (!ok) {
-    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 5);
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);
   }
   fence_before_sync();
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(256) gemm_tc_pair_dual_kernel(const __grid_con
   }
   __syncwarp();
   if (abort_s[half_no]) {
-    if ((tid & 127) == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+    if ((tid & 127) == 0 && p.error_flag) atomicExch(p.error_flag, 5);
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);
   }
   fence_before_sync();

@@ -38,12 +38,12 @@ __global__ void __launch_bounds__(256) kv8_stage_kernel(StageParams p) {
   const int* job = p.jobs + (size_t)blockIdx.x * kJobWords;
   const int slot = job[0], block = job[1], r0 = job[2], r1 = job[3], earlier = job[4], exact = job[5], last = job[6], last_rows = job[7];
   if (slot < 0 || slot >= p.n_slots || block < 0 || block >= p.max_blocks) {
-    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, kIndexOutside);
     return;
   }
   const int page = p.page_table[(size_t)slot * p.max_blocks + block];
   if (page < 0 || page >= p.n_pages) {
-    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+    if (tid == 0 && p.error_flag) atomicExch(p.error_flag, kIndexOutside);
     return;
   }
   const size_t cache_tile = ((size_t)page * p.n_kv_heads + head) * (PAGE * D), scale_at = (size_t)page * p.n_kv_heads + head;

@@ -149,13 +149,15 @@ def gemm_simt(a, w, out, mode=MODE_STORE, *, n_out=None, m_rows=None, a_rows=Non
           c_float(gate_limit), _stream())
 
 
-_errors = {}          # device index -> int32[2]: [0] a tensor-core kernel gave up a wait, [1] a token id out of range
+INDEX_OUTSIDE = 3     # word 0 of the error flags: an index outside of the cache (kIndexOutside in common.cuh)
+_errors = {}          # device index -> int32[2]: [0] a kernel gave up a wait or met an index outside of the cache, [1] a token id out of range
 
 
 def device_error_flags(device) -> torch.Tensor:
-    """int32[2] on the device that kernels write when something went wrong: word 0 is set to 1 by a tensor-core
-    kernel whose bounded barrier wait ran out, word 1 to 1 + t by the embedding kernel when token t of a step
-    was outside the vocabulary.  The engine reads and clears them."""
+    """int32[2] on the device that kernels write when something went wrong.  Word 0: INDEX_OUTSIDE by a kernel over the cache in
+    8 bits that met a position, slot or page outside of it; any other number (1, 2, 4, 5, by kind of kernel) by a kernel
+    whose bounded barrier wait ran out.  Word 1: 1 + t by the embedding kernel when token t of a step was outside the
+    vocabulary.  The engine reads and clears them."""
     idx = (device if isinstance(device, torch.device) else torch.device(device)).index or 0
     if idx not in _errors:
         _errors[idx] = torch.zeros(2, dtype=torch.int32, device=device)
@@ -163,7 +165,7 @@ def device_error_flags(device) -> torch.Tensor:
 
 
 def tc_error_flag(device) -> torch.Tensor:
-    """int32[1] that a tensor-core kernel sets when one of its bounded waits ran out."""
+    """int32[1], word 0 of `device_error_flags`."""
     return device_error_flags(device)[0:1]
 
 

@@ -279,12 +279,12 @@ class Engine:
             return
         ev.synchronize()
         self._err_copied = False
-        gave_up, token = int(self._err_host[0]), int(self._err_host[1])
+        gave_up, token = int(self._err_host[0]), int(self._err_host[1])       # (see device_error_flags)
         if not (gave_up or token):
             return
         self._err_dev.zero_()
         self._err_host.zero_()
-        if gave_up == 3:
+        if gave_up == K.INDEX_OUTSIDE:
             raise RuntimeError("attention: a position, slot or page of a step was outside of the cache; the results of the steps since the "
                                "last check are invalid")
         if gave_up:
