@@ -53,7 +53,8 @@ class Kv8Plan:
     Pages 0 .. n_earlier - 1 hold earlier blocks; pages n_earlier .. n_pages - 1 the blocks that the step's tokens fall into,
     sequence after sequence from each one's first new block on.  `exact_table` and `earlier_table` [sequences, width] name
     them per block (-1: none); a kernel that stores rows through a page table stores them through `exact_table` with
-    `seq_ids` as the sequences' slots."""
+    `seq_ids` as the sequences' slots.  `moved`: the slots whose tail the step gives to another block, or None: a caller that may
+    have to run the step again keeps those tails (`KeptTails`), as the rows in them are held nowhere else."""
 
     def __init__(self, starts, n_new, slots, *, window_kind: str = "full", window_size: int = 0, keep_first: int = 0, device="cuda"):
         if not len(starts) == len(n_new) == len(slots) or not len(starts):
@@ -98,7 +99,8 @@ class Kv8Plan:
             jobs.append(job)
         jobs = np.concatenate(jobs)
         self.n_pages, self.n_jobs = at, len(jobs)
-        flat = np.concatenate([tables.ravel(), np.arange(n, dtype=np.int32), jobs.ravel()])
+        moved = [slot for s, e, slot in zip(starts, ends, slots) if s % BLOCK and e % BLOCK and s // BLOCK != e // BLOCK]
+        flat = np.concatenate([tables.ravel(), np.arange(n, dtype=np.int32), jobs.ravel(), np.array(moved, dtype=np.int32)])
         host = torch.from_numpy(flat)
         dev = torch.device(device)
         if dev.type == "cuda":
@@ -106,4 +108,22 @@ class Kv8Plan:
         self._host, words = host, n * self.width
         d = host.to(dev, non_blocking=True)
         self.earlier_table, self.exact_table = d[:words].view(n, -1), d[words:2 * words].view(n, -1)
-        self.seq_ids, self.jobs = d[2 * words:2 * words + n], d[2 * words + n:]
+        self.seq_ids, self.jobs = d[2 * words:2 * words + n], d[2 * words + n:2 * words + n + jobs.size]
+        self.moved = d[2 * words + n + jobs.size:] if moved else None
+
+
+class KeptTails:
+    """Tails that a step gives to other blocks, kept until it is through: a step that fails on the way is undone."""
+
+    def __init__(self):
+        self._kept = []
+
+    def keep(self, cache: Kv8Cache, plan: Kv8Plan) -> None:
+        """Called before the step's first `kv8_stage`, for the cache of a layer or of many (tensors with one more axis in front)."""
+        if plan.moved is not None:
+            self._kept += [(t, plan.moved, t.index_select(t.dim() - 4, plan.moved)) for t in (cache.k_tail, cache.v_tail)]
+
+    def put_back(self) -> None:
+        for tails, slots, rows in self._kept:
+            tails.index_copy_(tails.dim() - 4, slots.long(), rows)
+        self._kept.clear()

@@ -331,6 +331,15 @@ class CacheManager:
             g.sync_tables()
         return starts
 
+    def keep_tails(self, batch) -> "kv8.KeptTails":
+        """Called before a step of several tokens per sequence runs: what the groups that are held in 8 bits have in the tails that the
+        step gives to other blocks.  (Rows in pages need no such care: a step that is run again stores them at the same places.)"""
+        tails = kv8.KeptTails()
+        for g in self.groups:
+            if g.kv8 is not None:
+                tails.keep(g.kv8, batch.kv8_plan(g.req.window_kind, g.req.window_size, g.req.keep_first))
+        return tails
+
     def commit_step(self, slots: list, n_new: list) -> None:
         for s, n in zip(slots, n_new):
             self.lengths[s] += n

@@ -1246,7 +1246,8 @@ def kv8_stage(cache, page_table, plan, k_pages, v_pages):
     """The pages of a step of several tokens (`plan`: a Kv8Plan): k_pages, v_pages bfloat16 [plan.n_pages, kv heads, 64,
     head_dim], whose exact pages hold the step's new rows already.  Fills in the rows before them from the tails and zeros
     behind them, writes the blocks that are complete now to the cache and each sequence's open block to its tail, and puts
-    the numbers that earlier blocks stand for into the earlier pages."""
+    the numbers that earlier blocks stand for into the earlier pages.  The tails of `plan.moved` hold another block after it: the
+    same step cannot be staged a second time unless they are put back (`cache.kv8.KeptTails`)."""
     what = "kv8_stage"
     fmt, nkv, d, slots, at = _kv8(cache, what)
     table, jobs = page_table.shape, plan.jobs

@@ -202,7 +202,13 @@ class Engine:
             batch = self.stager.stage(slots, starts, toks, wants, self.dtype)
             if device_tokens is not None:
                 batch.tokens.copy_(device_tokens.view(-1))
-            logits = self.model.run(batch, self.cache)
+            tails = None if decode else self.cache.keep_tails(batch)
+            try:
+                logits = self.model.run(batch, self.cache)
+            except BaseException:               # nothing is committed: the caller may run the step again, or a smaller one
+                if tails is not None:
+                    tails.put_back()
+                raise
         self.cache.commit_step(slots, n_new)
         self.steps_run += 1
         self._copy_error_flags()
