@@ -333,7 +333,9 @@ class CacheManager:
 
     def keep_tails(self, batch) -> "kv8.KeptTails":
         """Called before a step of several tokens per sequence runs: what the groups that are held in 8 bits have in the tails that the
-        step gives to other blocks.  (Rows in pages need no such care: a step that is run again stores them at the same places.)"""
+        step gives to other blocks.  (Rows in pages need no such care: a step that is run again stores them at the same places.)
+        It makes the step's plans too: their tables are index arrays, which kernels may read before they wait for the kernel in
+        front, so their copies end before the step's first kernel starts."""
         tails = kv8.KeptTails()
         for g in self.groups:
             if g.kv8 is not None:

@@ -90,3 +90,22 @@ def test_two_failures_in_a_row(monkeypatch):
                 e.step([StepEntry(slot, seqs[0][100:200], range(100))])
     assert torch.equal(want[1], e.step([StepEntry(slot, seqs[0][100:200], range(100))]))
     e.release_slot(slot)
+
+
+@pytest.mark.parametrize("name", ["dense", "beside", "turned"])
+def test_a_steps_plans_are_there_before_its_first_kernel(name, monkeypatch):
+    """Their tables are read by kernels that do not wait for the kernel in front first: no layer makes one."""
+    e = engine(name, "int8")
+    windows = {(g.req.window_kind, g.req.window_size, g.req.keep_first) for g in e.cache.groups if g.kv8 is not None}
+    whole, seen = e.model.run, []
+
+    def run(batch, cache):
+        seen.append(set(batch.plans))
+        made = dict(batch.plans)
+        logits = whole(batch, cache)
+        assert batch.plans.keys() == made.keys()
+        return logits
+
+    monkeypatch.setattr(e.model, "run", run)
+    steps(e, [tiny.random_tokens(200, vocab(name), 1)], [(100,), (50,), (50,)])
+    assert seen == [windows] * 3 and windows
