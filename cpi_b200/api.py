@@ -14,7 +14,7 @@ from typing import Callable, Optional, Sequence
 
 from .engine import Engine, GenerationRequest, GenerationResult, Generator, StepEntry
 from .sampling import SamplingParams
-from .engine.score import score_sequence
+from .engine.score import check_scored, score_sequence
 from .sampling.sampler import Sampler, TokenScore
 
 __all__ = ["Model", "generate", "GenerationResult", "SamplingParams", "TokenScore"]
@@ -109,8 +109,9 @@ class Model:
 
     def score(self, sequences: Sequence[Sequence[int]], top: int = 0) -> list:
         """How probable each token of the given sequences (two tokens or more each) was after those before it: per
-        sequence of n tokens n - 1 TokenScores, of its second token to its last."""
+        sequence of n tokens n - 1 TokenScores, of its second token to its last, each with the `top` (up to 32) most probable ones."""
         out = []
+        sequences = [check_scored(self.engine, tokens, top) for tokens in sequences]
         for tokens in sequences:
             got = score_sequence(self.engine, tokens, top)
             lp, entropy = got.logprob.tolist(), got.entropy.tolist()

@@ -1537,7 +1537,8 @@ def ban_tokens(logits, ids, id_offsets):
 
 
 @functools.lru_cache(maxsize=None)
-def _log_probs_most() -> int:
+def log_probs_most() -> int:
+    """The most alternatives that `log_probs` lists."""
     return int(load().cpi_log_probs_max_top())
 
 
@@ -1561,7 +1562,7 @@ def log_probs(logits, targets, *, top=0):
     if targets.dtype not in (torch.int32, torch.int64) or targets.dim() not in (1, 2) or targets.shape[0] != R or not targets.is_contiguous():
         raise KernelError(f"{what}: targets are contiguous int32 or int64 [{R}] or [{R}, n], not {targets.dtype} {tuple(targets.shape)}")
     top = int(top)
-    most = _log_probs_most()
+    most = log_probs_most()
     if not 0 <= top <= min(most, V):
         raise KernelError(f"{what}: top {top} of a vocabulary of {V} (at most {most})")
     here = _here(what, logits, targets)

@@ -19,6 +19,7 @@ from dataclasses import dataclass
 from typing import Callable, Optional, Sequence
 
 from ..sampling.params import SamplingParams, GREEDY
+from .score import most_alternatives
 
 
 @dataclass
@@ -111,8 +112,9 @@ class Generator:
             if r.max_new < 1:
                 raise ValueError(f"request {i}: max_new must be >= 1")
             r.sampling.validate()
-            if r.logprobs is not None and r.logprobs < 0:
-                raise ValueError(f"request {i}: logprobs must be a number of alternatives, 0 or more, not {r.logprobs}")
+            if r.logprobs is not None and not 0 <= r.logprobs <= most_alternatives(self.engine):
+                raise ValueError(f"request {i}: logprobs must be a number of alternatives from 0 to {most_alternatives(self.engine)}, "
+                                 f"not {r.logprobs}")
             reqs.append(GenerationRequest(prompt, r.max_new, r.sampling, r.stop_ids, r.logprobs))
         cache = self.engine.cache
         batches = plan_batches(reqs, max_batch=self.max_batch, token_capacity=cache.n_pages * cache.page_size,

@@ -16,20 +16,34 @@ from .engine import StepEntry
 LOGIT_BYTES = 1 << 30
 
 
+def most_alternatives(engine) -> int:
+    return min(K.log_probs_most(), engine.spec.vocab_size)
+
+
+def check_scored(engine, tokens: Sequence[int], top: int = 0) -> list:
+    """The tokens as a list, if they and `top` can be scored; a ValueError if not."""
+    tokens, vocab = [int(t) for t in tokens], engine.spec.vocab_size
+    if len(tokens) < 2:
+        raise ValueError("a sequence to score has two tokens or more: the first is given, the others are scored")
+    if min(tokens) < 0 or max(tokens) >= vocab:
+        raise ValueError(f"a token id lies outside the vocabulary of {vocab}")
+    if not 0 <= top <= most_alternatives(engine):
+        raise ValueError(f"scores list up to {most_alternatives(engine)} alternatives, not {top}")
+    return tokens
+
+
 def score_sequence(engine, tokens: Sequence[int], top: int = 0) -> "K.LogProbs":
     """Of tokens t_0 .. t_{n-1} (n >= 2) the log probabilities of t_1 .. t_{n-1} given what precedes each, the entropy of each
     distribution and its `top` best tokens: a LogProbs of n - 1 rows on the device."""
-    tokens = [int(t) for t in tokens]
-    if len(tokens) < 2:
-        raise ValueError("a sequence to score has two tokens or more: the first is given, the others are scored")
+    tokens = check_scored(engine, tokens, top)
     n = len(tokens) - 1
     piece = max(1, min(engine.max_step_tokens, LOGIT_BYTES // (4 * engine.spec.vocab_size)))
-    if min(tokens) < 0 or max(tokens) >= engine.spec.vocab_size:
-        raise ValueError(f"a token id lies outside the vocabulary of {engine.spec.vocab_size}")
-    targets = torch.tensor(tokens[1:], dtype=torch.int32, device=engine.device)
     slot = engine.acquire_slot()
     parts = []
     try:
+        # all pieces fit, or none runs
+        engine.cache.check_room([([slot], [min(piece, n - a)]) for a in range(0, n, piece)])
+        targets = torch.tensor(tokens[1:], dtype=torch.int32, device=engine.device)
         for a in range(0, n, piece):
             b = min(n, a + piece)
             logits = engine.step([StepEntry(slot, tokens[a:b], range(b - a))])
