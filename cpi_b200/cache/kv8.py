@@ -3,8 +3,10 @@
 Positions 64 b .. 64 b + 63 of a sequence are its block b, one page.  A complete block is held as codes of 8 bits with one
 power of two as scale per page and key/value head, keys and values each (an element stands for code * scale); the block of
 the newest position is held in bfloat16, in the sequence's *tail*, until it is complete.  A query sees the keys and values
-of its own block in bfloat16 and those of earlier blocks as held in 8 bits, whatever step brought them: a position's result
-does not depend on how its sequence was cut into steps.
+of its own block in bfloat16 and those of earlier blocks as held in 8 bits, whatever step brought them: what a position
+attends to does not depend on how its sequence was cut into steps.  (Its numbers may by a rounding: other steps project rows by
+products of other shapes, and single tokens and prompts round probabilities differently.  Values have to be finite: one that is not
+also reaches earlier queries of its sequence within a prompt's key tile.)
 
   "int8"   scale = the smallest power of two with max |x| <= 127 scale; code = x / scale to the nearest integer
   "e4m3"   max |x| / scale in [128, 256); code = x / scale to the nearest e4m3 number
@@ -49,6 +51,9 @@ def needed_blocks(start: int, new: int, window_kind: str, window_size: int, keep
 class Kv8Plan:
     """Where a step's tokens and the blocks that they see lie among the step's own bfloat16 pages.  Made once per step and
     window (`starts`, `n_new`, `slots` per sequence, as in a StepBatch), used by every layer with that window.
+
+    The pages hold all that the step's sequences see in bfloat16, 4 x kv heads x head size bytes a position, while a layer's
+    attention runs.
 
     Pages 0 .. n_earlier - 1 hold earlier blocks; pages n_earlier .. n_pages - 1 the blocks that the step's tokens fall into,
     sequence after sequence from each one's first new block on.  `exact_table` and `earlier_table` [sequences, width] name

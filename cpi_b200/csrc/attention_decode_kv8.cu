@@ -25,7 +25,8 @@
 // (bfloat16 would keep 8 bits of all of them, but codes cost twice as many operations to become bfloat16.)  Sums, maxima and
 // outputs are float32.
 //
-// The tail: four warps take 16 positions each in bfloat16, straight from memory (one page at most, in the last split).  A token
+// The tail: four warps take 16 positions each in bfloat16, straight from memory (one page at most, in the last split); its p is
+// bfloat16 like the values that it is multiplied by (outputs are off by 0.0016 to 0.0018, what rounding them takes is 0.0016).  A token
 // that completes its block (position 63 of 64) has its tail turned into codes, for the steps after this one, by the last split.
 // Rows of masked positions are zeros before they are multiplied: what an earlier sequence left cannot reach a result.
 // Waits are bounded as in attention_decode.cu.

@@ -21,9 +21,12 @@
 // reference m is its first tile's maximum, raised (and O rescaled in tensor memory) only when the row maximum has outgrown it by
 // 2^40: P is bfloat16 and the sums are float32, which have the same range of powers, so nothing is lost by numbers up to 2^40 (sums up
 // to 2^57, outputs finite for values up to 2^70), and it happens in a row's first tile and hardly ever again (keys and queries with a
-// few large features, 3,001 tokens of 40 heads: 190 us with 2^8, 171 with 2^40).  Tiles without a mask are taken into registers
-// whole, the maximum first, then P and the sum with two numbers to an instruction.  Masked tiles, and those that outgrow a reference,
-// go by 32 columns with the next ones on their way, against the reference they have; what has been stored of a tile's P is rescaled
+// few large features, 3,001 tokens of 40 heads: 190 us with 2^8, 171 with 2^40).  P has 8 bits because the A operand of a product
+// with bfloat16 values is bfloat16: outputs are off by 0.0021 to 0.0023 of their size where rounding the output alone takes 0.0016
+// (the rest of P as a second operand would double the value products); row sums take the weights unrounded.
+// Tiles without a mask are taken into registers whole, the maximum first, then P and the sum with two numbers to an instruction.
+// Masked tiles, and those that outgrow a reference, go by 32 columns with the next ones on their way, against the reference they
+// have; what has been stored of a tile's P is rescaled
 // too.  Columns that no row of the warp sees are passed over.
 //
 // Bound by the chain S -> softmax -> P V -> next S of each query tile (about 3,600 cycles for two tiles of 128 x 128, where the products

@@ -49,7 +49,12 @@ class Engine:
                  max_seqs: Optional[int] = None, max_seq_len: Optional[int] = None, page_size: int = 64,
                  max_step_tokens: int = 8192, config=None, cache_dtype: Optional[str] = None):
         """`cache_dtype`: "int8" or "e4m3" holds the keys and values of the attention layers in 8 bits (cache/kv8.py);
-        default: in `dtype`."""
+        default: in `dtype`.  Every one of `max_seqs` slots then has a block of 64 positions in bfloat16 per layer (name the number: the
+        default, a slot per page, takes more than 8 bits save), and a step of several tokens holds the past that its sequences see in
+        bfloat16, one layer at a time, which `max_tokens` and `max_step_tokens` do not count.
+
+        A step that raises has committed nothing: attention layers read what they would have read before it.  (Layers with a
+        state, recurrences and short convolutions, change it in place: their sequences start again.)"""
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise RuntimeError("cpi_b200 runs on a CUDA device only; there is no CPU path")

@@ -1,6 +1,7 @@
 """Scores of given tokens: a sequence is run as a prompt, and every position's logits say how probable the next token was.
 
-The logits of a piece (float32 [tokens, vocab]) live in one buffer; pieces are cut so that it stays below LOGIT_BYTES.  Each
+The logits of a piece (float32 [tokens, vocab]) live in one buffer of the engine's, which keeps the size that its largest step
+needed; pieces are cut so that it stays below LOGIT_BYTES.  Each
 piece's rows go through one launch of `log_probs`; nothing else of them is kept.  (The reference scores nothing: it prints the
 largest logits after a prompt, src/engine/llama4_cuda_engine.cu:623-674.)
 """
