@@ -76,14 +76,15 @@ constexpr int kIndexOutside = 3;
 // precedes the wait (barrier set-up, tensor-memory allocation, loads of weights, which no kernel writes) overlaps the
 // predecessor's tail.
 // Two things besides weights are read before the wait, by few kernels and under a condition each.  A step's index arrays
-// (positions, slots, page tables, runs of tokens, the tables of a plan over the cache in 8 bits) come from copies that end before
-// the step's first kernel starts (CacheManager.keep_tails has the plans made): read by attention_decode, qkv_post_d128,
-// qkv_conv_rotate and head_turn.  Cached pages, all but the one that holds the newest position: read by attention_decode.  Their rows come from earlier launches, each of which an attention kernel followed, and those that read
-// cached keys let their successors start only after their own wait, when the rows have been stored: whatever starts later
-// finds them.  So steps may follow one another without anything between them; but between a launch that stores several
-// positions of a sequence and attention_decode over that sequence there has to be such a kernel or a full stop.  (Letting
-// successors start after the wait in the kernels that store the rows instead takes as much from attention_decode's early
-// start as the page loads gain: 9 to 17 tokens of 40 heads 3 to 4 us of 40 to 64.)
+// (positions, slots, page tables, runs of tokens, the tables of a plan over the cache in 8 bits) come from copies that
+// end before the step's first kernel starts (CacheManager.keep_tails has the plans made): read by attention_decode,
+// qkv_post_d128, qkv_conv_rotate and head_turn.  Cached pages, all but the one that holds the newest position: read by
+// attention_decode.  Their rows come from earlier launches, each of which an attention kernel followed, and those that
+// read cached keys let their successors start only after their own wait, when the rows have been stored: whatever starts
+// later finds them.  So steps may follow one another without anything between them; but between a launch that stores
+// several positions of a sequence and attention_decode over that sequence there has to be such a kernel or a full stop.
+// (Letting successors start after the wait in the kernels that store the rows instead takes as much from
+// attention_decode's early start as the page loads gain: 9 to 17 tokens of 40 heads 3 to 4 us of 40 to 64.)
 // A kernel that allocates tensor memory lets its successors start only when it has it.  Before, a successor's block that
 // fits the same SM could take the columns first and keep them until this kernel ends, which waits for those columns.  With
 // that order whoever holds columns belongs to a kernel that is wholly resident, has all it needs and waits for earlier

@@ -10,7 +10,8 @@ stops leaves the next step's batch and gives its slot back at once, and when mor
 than fit, batch follows batch in slots that the previous one freed.
 
 The loop talks to the engine through four calls (acquire_slot, release_slot, step, length) and to a
-sampler through one, so its decisions can be tested without a device.
+sampler through one, so its decisions can be tested without a device.  (Requests that ask for log probabilities also
+need the engine's vocabulary size and the sampler's scores.)
 """
 from __future__ import annotations
 
