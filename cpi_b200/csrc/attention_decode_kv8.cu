@@ -766,8 +766,8 @@ extern "C" int cpi_attention_decode_kv8_supported(int n_heads, int n_kv_heads, i
 
 // Whether `n_splits` blocks of threads for each of `base` (token, kv head) pairs are joined within the kernel, as clusters, or
 // through scratch by a second one.  A cluster saves a launch and the scratch, but its blocks stay until the last of them is
-// through: 160 blocks (5 windowed sequences, 8 kv heads of 64) take 7.3 us as clusters and 7.4 with the second kernel, 256 (8 x 4,096
-// positions, 8 kv heads of 128) 23.2 and 21.3, 1,536 (64 sequences) 201 and 188.
+// through: 160 blocks (5 windowed sequences, 8 kv heads of 64) take 7.9 us as clusters and 8.1 with the second kernel, 256 (8 x 4,096
+// positions, 8 kv heads of 128) 23.8 and 22.5, 1,536 (64 sequences) 203 and 190.
 extern "C" int cpi_attention_decode_kv8_clustered(int base, int n_splits) {
   return n_splits > 1 && n_splits <= dec8::kMaxCluster && 3l * base * n_splits <= 4l * sm_count();
 }
